@@ -27,6 +27,9 @@ if EXPERIMENTS:
 EXTRA_FLAGS = {"attention.hip": ["-fno-honor-nans"]}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
+# no packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): hipcc -O3 makes it from ordinary float code, and on these machines some of its
+# forms have given wrong results now and then, without an error.  (hipcc's host pass warns that it does not know the feature: harmless.)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 RZ_F32, RZ_BF16, RZ_F16 = 0, 1, 2
 PROF_FAMILIES = ("attn", "gemm", "rowops", "vlcabs", "post")
@@ -52,7 +55,7 @@ def _source_digest() -> str:
     depend on file times — a snapshot copied to another machine (gpurun, the driver's round-end run) keeps contents, not necessarily mtime order."""
     import hashlib
     h = hashlib.sha256()
-    h.update(("experiments" if EXPERIMENTS else "product").encode() + os.environ.get("RZ_CXXFLAGS", "").encode())
+    h.update(("experiments" if EXPERIMENTS else "product").encode() + os.environ.get("RZ_CXXFLAGS", "").encode() + " ".join(NO_PACKED_F32).encode())
     for d in sorted(os.path.abspath(p) for p in _all_deps() if os.path.isfile(p)):
         h.update(os.path.basename(d).encode())
         with open(d, "rb") as f:
@@ -101,20 +104,24 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 def _build_locked(obj_dir: str, verbose: bool, force: bool = False) -> str:
     flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Werror=uninitialized",
-             "-Werror=return-type", f"-I{CSRC}"] + (["-DRZ_EXPERIMENTS", f"-I{EXP_SRC}"] if EXPERIMENTS else []) + os.environ.get("RZ_CXXFLAGS", "").split()   # RZ_CXXFLAGS: A/B builds of a tunable (with RZ_LIB_PATH)
+             "-Werror=return-type", *NO_PACKED_F32, f"-I{CSRC}"] + (["-DRZ_EXPERIMENTS", f"-I{EXP_SRC}"] if EXPERIMENTS else []) + os.environ.get("RZ_CXXFLAGS", "").split()   # RZ_CXXFLAGS: A/B builds of a tunable (with RZ_LIB_PATH)
     tag = f".{os.getpid()}.tmp"
 
     def cc(src):
         obj = os.path.join(obj_dir, src.replace(".hip", ".o"))
-        if not force and os.path.exists(obj) and os.path.getmtime(obj) > _src_mtime(src):
-            return obj                                   # unchanged translation unit: keep its object
-        cmd = [HIPCC, *flags, *EXTRA_FLAGS.get(src, []), "-c", _src_path(src), "-o", obj + tag]
+        cmd = [HIPCC, *flags, *EXTRA_FLAGS.get(src, []), "-c", _src_path(src), "-o"]
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) > _src_mtime(src) and _read(obj + ".cmd") == " ".join(cmd):
+            return obj                                   # unchanged translation unit, same command: keep its object
+        cmd.append(obj + tag)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"hipcc failed for {src}:\n{r.stderr}")
         if r.stderr and (verbose or "-Wuninitialized" in r.stderr or "-Wreturn-type" in r.stderr or "-Wsometimes-uninitialized" in r.stderr):
             print(r.stderr, file=sys.stderr)         # these warnings have been real bugs: never hide them
         os.replace(obj + tag, obj)
+        with open(obj + ".cmd" + tag, "w") as f:
+            f.write(" ".join(cmd[:-1]))
+        os.replace(obj + ".cmd" + tag, obj + ".cmd")
         return obj
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
@@ -128,6 +135,14 @@ def _build_locked(obj_dir: str, verbose: bool, force: bool = False) -> str:
         f.write(_source_digest() + "\n")
     os.replace(STAMP_PATH + tag, STAMP_PATH)
     return LIB_PATH
+
+
+def _read(path: str) -> str:
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return ""
 
 
 def _src_mtime(src: str) -> float:
