@@ -230,6 +230,79 @@ int rz_image_features(const float* tokens_dev, int64_t image_stride_rows, int ba
 int rz_patch_embed(int dtype, const float* pixel_values_dev, int batch, int channels, int height, int width, int patch, const void* weight_dev,
                    int k_pad, const float* table_dev, int n_pad, void* im2col_ws_dev, float* out_dev, void* stream);
 
+/* ---- operators of a differential-attention block: rotary positions -> differential attention -> (rz_gemm) -> norms with gate and residual ----
+ * Arguments in a struct, copied before the call returns.  Strides are in elements; columns are contiguous.  No workspace is kept between
+ * calls, no call waits for the device, every call may be captured.  Forward only.
+ *
+ * Rotary positions: every pair (u, w) of a head turns by angle = position * freq to amplitude * (u cos - w sin, u sin + w cos).
+ *   layout RZ_ROTARY_HALF: u = x[p], w = x[p + rotary_dim / 2]; RZ_ROTARY_INTERLEAVED: u = x[2 p], w = x[2 p + 1]; p = 0 .. rotary_dim / 2 - 1;
+ *   columns from rotary_dim (even, <= head_dim <= 1024) on pass through.  k_heads = 0: q alone.
+ *   positions_dev int64, axis x of token n of batch entry b at [b * positions_batch_stride + n * positions_token_stride + x] (any sign, |position| < 2^31;
+ *   a batch stride of 0 shares them); freqs_dev double (rotary_dim / 2): radians per position, pairs dealt to the n_axes axes in equal runs.
+ *   Outputs may be the inputs themselves (in place, same strides); they may not overlap them otherwise. */
+enum rz_rotary_layout { RZ_ROTARY_HALF = 0, RZ_ROTARY_INTERLEAVED = 1 };
+typedef struct rz_rotary_args {
+    int32_t dtype, layout, batch, tokens, q_heads, k_heads, head_dim, rotary_dim, n_axes;
+    float amplitude;
+    const void* q_dev; int64_t q_batch_stride, q_token_stride, q_head_stride;
+    const void* k_dev; int64_t k_batch_stride, k_token_stride, k_head_stride;
+    void* q_out_dev; int64_t q_out_batch_stride, q_out_token_stride, q_out_head_stride;
+    void* k_out_dev; int64_t k_out_batch_stride, k_out_token_stride, k_out_head_stride;
+    const int64_t* positions_dev; int64_t positions_batch_stride, positions_token_stride;
+    const double* freqs_dev;
+} rz_rotary_args;
+int rz_rotary(const rz_rotary_args* args, void* stream);
+
+/* Differential attention: out = out_scale * norm((softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v),
+ *   lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init.
+ *   A head's row of q and k is [first map | second map], head_dim each (32, 64 or 128); its row of v and out has 2 * head_dim columns.  heads is a
+ *   multiple of kv_heads; query head h reads key head h / (heads / kv_heads).  q, k, v, out: 16-byte aligned, strides multiples of 16 bytes.
+ *   lambda_qk_dev fp32 (4, head_dim) = lq1 | lk1 | lq2 | lk2 for every head (lambda_head_stride 0) or per query head (its stride).
+ *   norm_weight_dev fp32 (2 head_dim) = root-mean-square norm of each output row (eps norm_eps), NULL = none.
+ *   Which keys a query sees: kv_lens_dev int32 (batch) = the first kv_lens[b] keys (clamped to 0 .. n_k), NULL = n_k of them; mask_dev int64
+ *   (batch, n_k), 0 = hidden, NULL = none (the tokenizer's attention_mask as it comes); causal RZ_CAUSAL_START: query i is token i and sees keys
+ *   0 .. i; RZ_CAUSAL_END: the queries are the last n_q tokens of their sequence, query i sees keys 0 .. len - n_q + i.  A query that sees no key
+ *   gets zeros.  What a hidden key holds, inf and NaN included, changes nothing.
+ *   Statistics and sums are fp32; the 16-bit types round each weight exp(s - max) to the type for the product with v.
+ *   workspace_dev: rz_diff_attention_workspace(args) bytes (0: may be NULL), 16-byte aligned, free for reuse when the call's kernels are done. */
+enum rz_causal { RZ_CAUSAL_NONE = 0, RZ_CAUSAL_START = 1, RZ_CAUSAL_END = 2 };
+typedef struct rz_diff_attention_args {
+    int32_t dtype, batch, heads, kv_heads, n_q, n_k, head_dim, causal;
+    float scale, lambda_init, norm_eps, out_scale;
+    const void* q_dev; int64_t q_batch_stride, q_token_stride, q_head_stride;
+    const void* k_dev; int64_t k_batch_stride, k_token_stride, k_head_stride;
+    const void* v_dev; int64_t v_batch_stride, v_token_stride, v_head_stride;
+    void* out_dev; int64_t out_batch_stride, out_token_stride, out_head_stride;
+    const float* lambda_qk_dev; int64_t lambda_head_stride;
+    const float* norm_weight_dev;
+    const int32_t* kv_lens_dev;
+    const int64_t* mask_dev; int64_t mask_batch_stride;
+} rz_diff_attention_args;
+/* bytes of workspace_dev the call below needs for these sizes (0 also on a bad argument, which the call itself reports) */
+size_t rz_diff_attention_workspace(const rz_diff_attention_args* args);
+int rz_diff_attention(const rz_diff_attention_args* args, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* The norms either side of a block with its gate and residual scale: t = post_norm(y); r = alpha * resid + scale * gate * t -> resid_out;
+ *   pre_norm(r) -> out (the next block's operand).  y_dev, out_dev `dtype`; resid `resid_dtype` (RZ_F32 or `dtype`); everything else fp32.
+ *   y_dev NULL: r = alpha * resid.  resid_out_dev / out_dev NULL: not written (not both); resid_out_dev may be resid_dev, out_dev may be y_dev or, of
+ *   one type, resid_dev (same strides).  Norm kinds: RZ_NORM_NONE, RZ_NORM_LAYER, RZ_NORM_RMS; weights and biases (dim) or NULL; scale_dev (dim) or NULL;
+ *   gate_dev row of batch entry b, row n at b * gate_batch_stride + n * gate_row_stride (0 = shared), or NULL.  1 <= dim <= 16384, any alignment.
+ *   The statistics of pre_norm are those of r in fp32, before it is rounded to resid_dtype. */
+enum rz_norm_kind { RZ_NORM_NONE = 0, RZ_NORM_LAYER = 1, RZ_NORM_RMS = 2 };
+typedef struct rz_residual_norm_args {
+    int32_t dtype, resid_dtype, batch, rows, dim, post_kind, pre_kind;
+    float alpha, post_eps, pre_eps;
+    const void* y_dev; int64_t y_batch_stride, y_row_stride;
+    const void* resid_dev; int64_t resid_batch_stride, resid_row_stride;
+    void* resid_out_dev; int64_t resid_out_batch_stride, resid_out_row_stride;
+    void* out_dev; int64_t out_batch_stride, out_row_stride;
+    const float* post_weight_dev; const float* post_bias_dev;
+    const float* scale_dev;
+    const float* gate_dev; int64_t gate_batch_stride, gate_row_stride;
+    const float* pre_weight_dev; const float* pre_bias_dev;
+} rz_residual_norm_args;
+int rz_residual_norm(const rz_residual_norm_args* args, void* stream);
+
 /* fp32 GEMM on the f16 / fp8 matrix pipes, kernel level — the two operand forms of the fp32 (1e-3) mode's vision encoder
  * (TF:dinov2/modeling_dinov2.py:199-213, :246-251, :281-297 computed with fp32 inputs): out_dev[m][n] += a[m][:] . w[n][:] + bias[n], fp32 `out_dev`
  * read-modify-write.  form 0 = every product as three f16 MFMAs over hi/lo planes; form 1 = "MX": a_hi b_hi on the f16 pipe + the two correction

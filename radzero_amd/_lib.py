@@ -17,7 +17,7 @@ EXP_SRC = os.path.join(PKG_DIR, "..", "tools", "experiments")     # retired expe
 # its own library and object directory; the product and every test use the plain build.
 EXPERIMENTS = os.environ.get("RZ_EXPERIMENTS") == "1"
 LIB_PATH = os.environ.get("RZ_LIB_PATH") or os.path.join(PKG_DIR, "libradzero_hip_experiments.so" if EXPERIMENTS else "libradzero_hip.so")   # RZ_LIB_PATH: A/B of two builds in one gpurun call
-SOURCES = ["gemm.hip", "gemm7.hip", "gemm8.hip", "attention.hip", "rowops.hip", "vlcabs.hip", "preprocess.hip", "api.hip"]
+SOURCES = ["gemm.hip", "gemm7.hip", "gemm8.hip", "attention.hip", "rowops.hip", "vlcabs.hip", "preprocess.hip", "rotary.hip", "diff_attention.hip", "residual_norm.hip", "api.hip"]
 if EXPERIMENTS:
     # retired GEMM experiments, never faster than gemm8 inside the step: gemm10 / gemm11 (round 3: other K loops), gemm12 (round 4: two
     # 256x128 workgroups per CU so that epilogues overlap K loops; profiles/r04/gemm12_*.log).  They live in tools/experiments/ (with the
@@ -170,6 +170,32 @@ class RzConfig(ctypes.Structure):
     ]
 
 
+def _struct(name, doc, *fields):
+    """A ctypes mirror of a C struct: "type name name ..." per line, types as in include/radzero_hip.h (i int32, f float, l int64, p pointer)."""
+    t = {"i": ctypes.c_int32, "f": ctypes.c_float, "l": ctypes.c_int64, "p": ctypes.c_void_p}
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": [(n, t[f.split()[0]]) for f in fields for n in f.split()[1:]]})
+
+
+RzRotaryArgs = _struct(
+    "RzRotaryArgs", "rz_rotary_args (include/radzero_hip.h)",
+    "i dtype layout batch tokens q_heads k_heads head_dim rotary_dim n_axes", "f amplitude",
+    "p q_dev", "l q_batch_stride q_token_stride q_head_stride", "p k_dev", "l k_batch_stride k_token_stride k_head_stride",
+    "p q_out_dev", "l q_out_batch_stride q_out_token_stride q_out_head_stride", "p k_out_dev", "l k_out_batch_stride k_out_token_stride k_out_head_stride",
+    "p positions_dev", "l positions_batch_stride positions_token_stride", "p freqs_dev")
+RzDiffAttentionArgs = _struct(
+    "RzDiffAttentionArgs", "rz_diff_attention_args (include/radzero_hip.h)",
+    "i dtype batch heads kv_heads n_q n_k head_dim causal", "f scale lambda_init norm_eps out_scale",
+    "p q_dev", "l q_batch_stride q_token_stride q_head_stride", "p k_dev", "l k_batch_stride k_token_stride k_head_stride",
+    "p v_dev", "l v_batch_stride v_token_stride v_head_stride", "p out_dev", "l out_batch_stride out_token_stride out_head_stride",
+    "p lambda_qk_dev", "l lambda_head_stride", "p norm_weight_dev kv_lens_dev mask_dev", "l mask_batch_stride")
+RzResidualNormArgs = _struct(
+    "RzResidualNormArgs", "rz_residual_norm_args (include/radzero_hip.h)",
+    "i dtype resid_dtype batch rows dim post_kind pre_kind", "f alpha post_eps pre_eps",
+    "p y_dev", "l y_batch_stride y_row_stride", "p resid_dev", "l resid_batch_stride resid_row_stride",
+    "p resid_out_dev", "l resid_out_batch_stride resid_out_row_stride", "p out_dev", "l out_batch_stride out_row_stride",
+    "p post_weight_dev post_bias_dev scale_dev gate_dev", "l gate_batch_stride gate_row_stride", "p pre_weight_dev pre_bias_dev")
+
+
 # every symbol include/radzero_hip.h declares: name -> (restype, argtypes)
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 SYMBOLS = {
@@ -207,6 +233,10 @@ SYMBOLS = {
     "rz_rows_dot": (_I, [_P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _L, _L, _L, _P]),
     "rz_image_features": (_I, [_P, _L, _I, _I, _I, _P, _P]),
     "rz_patch_embed": (_I, [_I, _P, _I, _I, _I, _I, _I, _P, _I, _P, _I, _P, _P, _P]),
+    "rz_rotary": (_I, [ctypes.POINTER(RzRotaryArgs), _P]),
+    "rz_diff_attention_workspace": (ctypes.c_size_t, [ctypes.POINTER(RzDiffAttentionArgs)]),
+    "rz_diff_attention": (_I, [ctypes.POINTER(RzDiffAttentionArgs), _P, ctypes.c_size_t, _P]),
+    "rz_residual_norm": (_I, [ctypes.POINTER(RzResidualNormArgs), _P]),
     "rz_set_option": (_I, [ctypes.c_char_p, _I]),
     "rz_set_model_option": (_I, [_P, ctypes.c_char_p, _I]),
     "rz_get_model_option": (_I, [_P, ctypes.c_char_p, ctypes.POINTER(_I)]),

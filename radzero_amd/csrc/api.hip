@@ -1674,6 +1674,72 @@ int rz_patch_embed(int dtype, const float* px, int B, int C, int Himg, int Wimg,
     return 0;
 }
 
+int rz_rotary(const rz_rotary_args* a, void* stream) {
+    if (!a) return fail(RZ_ERR_INVALID, "rz_rotary: null argument");
+    if (a->dtype < 0 || a->dtype > 2) return fail(RZ_ERR_INVALID, "rz_rotary: dtype");
+    if (a->layout != RZ_ROTARY_HALF && a->layout != RZ_ROTARY_INTERLEAVED) return fail(RZ_ERR_INVALID, "rz_rotary: layout");
+    if (a->batch < 0 || a->tokens < 0 || a->q_heads < 1 || a->k_heads < 0 || a->q_heads > 65536 || a->k_heads > 65536)
+        return fail(RZ_ERR_INVALID, "rz_rotary: bad shape");
+    if (a->head_dim < 2 || a->head_dim > 1024 || a->rotary_dim < 2 || a->rotary_dim > a->head_dim || a->rotary_dim % 2)
+        return fail(RZ_ERR_INVALID, "rz_rotary: rotary_dim must be even, 2 .. head_dim, head_dim at most 1024");
+    if (a->n_axes < 1 || (a->rotary_dim / 2) % a->n_axes) return fail(RZ_ERR_INVALID, "rz_rotary: the rotary pairs must be a multiple of the axes");
+    if (a->batch == 0 || a->tokens == 0) return 0;
+    if ((int64_t)a->batch * a->tokens > INT32_MAX) return fail(RZ_ERR_INVALID, "rz_rotary: too many tokens");
+    if (!a->q_dev || !a->q_out_dev || (a->k_heads && (!a->k_dev || !a->k_out_dev)) || !a->positions_dev || !a->freqs_dev)
+        return fail(RZ_ERR_INVALID, "rz_rotary: null pointer");
+    RZ_HIP(launch_rotary(*a, (hipStream_t)stream));
+    return 0;
+}
+
+static const char* diff_attention_error(const rz_diff_attention_args* a) {
+    if (!a) return "rz_diff_attention: null argument";
+    if (a->dtype < 0 || a->dtype > 2) return "rz_diff_attention: dtype";
+    if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) return "rz_diff_attention: head_dim must be 32, 64 or 128";
+    if (a->batch < 0 || a->n_q < 0 || a->n_k < 0 || a->heads < 1 || a->kv_heads < 1) return "rz_diff_attention: bad shape";
+    if (a->heads % a->kv_heads) return "rz_diff_attention: heads must be a multiple of kv_heads";
+    if (a->causal < RZ_CAUSAL_NONE || a->causal > RZ_CAUSAL_END) return "rz_diff_attention: causal";
+    if (!(a->scale > 0.f) || a->scale > 1e30f) return "rz_diff_attention: scale must be positive and finite";
+    if (a->norm_weight_dev && !(a->norm_eps >= 0.f)) return "rz_diff_attention: norm_eps must not be negative";
+    // 32-bit row numbers and grids inside; offsets are 64-bit
+    if (a->n_k > (1 << 30) || (int64_t)a->n_q * a->heads > (1 << 30) || (int64_t)a->batch * a->heads * a->n_q > INT32_MAX)
+        return "rz_diff_attention: too many rows";
+    return nullptr;
+}
+
+size_t rz_diff_attention_workspace(const rz_diff_attention_args* a) { return diff_attention_error(a) || !a->batch || !a->n_q ? 0 : diff_attention_workspace_bytes(*a); }
+
+int rz_diff_attention(const rz_diff_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    if (const char* e = diff_attention_error(a)) return fail(RZ_ERR_INVALID, e);
+    if (a->batch == 0 || a->n_q == 0) return 0;
+    if (!a->q_dev || !a->out_dev || !a->lambda_qk_dev || (a->n_k && (!a->k_dev || !a->v_dev))) return fail(RZ_ERR_INVALID, "rz_diff_attention: null pointer");
+    const int64_t m = a->dtype == RZ_F32 ? 4 : 8;
+    if (((uintptr_t)a->q_dev | (uintptr_t)a->k_dev | (uintptr_t)a->v_dev | (uintptr_t)a->out_dev | (uintptr_t)workspace) % 16 || a->q_batch_stride % m ||
+        a->q_token_stride % m || a->q_head_stride % m || a->k_batch_stride % m || a->k_token_stride % m || a->k_head_stride % m || a->v_batch_stride % m ||
+        a->v_token_stride % m || a->v_head_stride % m || a->out_batch_stride % m || a->out_token_stride % m || a->out_head_stride % m)
+        return fail(RZ_ERR_INVALID, "rz_diff_attention: q, k, v, out and their strides must be multiples of 16 bytes");
+    const size_t need = diff_attention_workspace_bytes(*a);
+    if (need && (!workspace || workspace_bytes < need)) return fail(RZ_ERR_STATE, "rz_diff_attention: workspace too small (rz_diff_attention_workspace)");
+    RZ_HIP(launch_diff_attention(*a, workspace, (hipStream_t)stream));
+    return 0;
+}
+
+int rz_residual_norm(const rz_residual_norm_args* a, void* stream) {
+    if (!a) return fail(RZ_ERR_INVALID, "rz_residual_norm: null argument");
+    if (a->dtype < 0 || a->dtype > 2 || (a->resid_dtype != RZ_F32 && a->resid_dtype != a->dtype))
+        return fail(RZ_ERR_INVALID, "rz_residual_norm: resid_dtype must be fp32 or dtype");
+    if (a->batch < 0 || a->rows < 0) return fail(RZ_ERR_INVALID, "rz_residual_norm: bad shape");
+    if (a->dim < 1 || a->dim > 16384) return fail(RZ_ERR_INVALID, "rz_residual_norm: dim must be 1 .. 16384");
+    if (a->post_kind < RZ_NORM_NONE || a->post_kind > RZ_NORM_RMS || a->pre_kind < RZ_NORM_NONE || a->pre_kind > RZ_NORM_RMS)
+        return fail(RZ_ERR_INVALID, "rz_residual_norm: norm kind");
+    if (!(a->post_eps >= 0.f) || !(a->pre_eps >= 0.f)) return fail(RZ_ERR_INVALID, "rz_residual_norm: eps must not be negative");
+    if (a->batch == 0 || a->rows == 0) return 0;
+    if (!a->resid_dev || (!a->resid_out_dev && !a->out_dev)) return fail(RZ_ERR_INVALID, "rz_residual_norm: null pointer");
+    if (!a->y_dev && (a->post_kind || a->scale_dev || a->gate_dev)) return fail(RZ_ERR_INVALID, "rz_residual_norm: post norm, scale and gate need y");
+    if ((int64_t)a->batch * a->rows > INT32_MAX) return fail(RZ_ERR_INVALID, "rz_residual_norm: too many rows");
+    RZ_HIP(launch_residual_norm(*a, (hipStream_t)stream));
+    return 0;
+}
+
 int rz_debug_buffer(const char* what, void* dev_ptr) {
     if (!what) return fail(RZ_ERR_INVALID, "rz_debug_buffer: null name");
 #ifdef RZ_EXPERIMENTS

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../../include/radzero_hip.h"
+
 namespace rz {
 
 enum Epilogue : int {
@@ -180,6 +182,12 @@ hipError_t launch_preprocess(const void* img, int src_dtype, int H, int W, int C
 size_t preprocess_batch_desc_bytes(int n);
 hipError_t launch_preprocess_batch(const void* descs_host, int n, int max_ph, int S, const float* mean, const float* stdv, float rescale,
                                    unsigned char* ws, float* out, int minmax_normalize, hipStream_t s);
+
+// operators of a differential-attention block; arguments as the C-ABI takes them, checked by api.hip
+hipError_t launch_rotary(const rz_rotary_args& a, hipStream_t s);
+size_t diff_attention_workspace_bytes(const rz_diff_attention_args& a);
+hipError_t launch_diff_attention(const rz_diff_attention_args& a, void* ws, hipStream_t s);
+hipError_t launch_residual_norm(const rz_residual_norm_args& a, hipStream_t s);
 
 // strided gather of valid tokens: src [B][Npad][D] -> dst [B][N][D]
 hipError_t launch_copy_tokens(const float* src, float* dst, int B, int n_valid, int n_pad, int D, hipStream_t s, const unsigned* run_if = nullptr);

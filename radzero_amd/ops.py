@@ -1,0 +1,269 @@
+"""Operators of a differential-attention block on torch tensors: rotary positions, differential attention, and the norms either side of a
+block with its gate and residual scale (rz_rotary, rz_diff_attention, rz_residual_norm of include/radzero_hip.h).
+
+They work on GPU tensors alone, on the current stream of the tensors' device, never wait for it and may be captured into a graph.  They are
+forward only, like everything here: an input that asks for a gradient is refused.  Types are float32, bfloat16 and float16 for tokens;
+weights, gates and lambda vectors are float32.  Strides are free except that columns are contiguous; what a kernel cannot take raises ValueError.
+
+    freqs, amplitude = rotary_frequencies(64, axes=2, device="cuda")
+    q, k = rotary(q, k, positions=patch_rows_and_columns, freqs=freqs, amplitude=amplitude)
+    ctx = diff_attention(q, k, v, lambda_qk, lambda_init=0.2, norm_weight=w, out_scale=0.8)
+    h, xn = residual_norm(h, out_projection, scale=layer_scale, pre_norm=Norm(weight, bias))
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.RZ_F32, torch.bfloat16: _lib.RZ_BF16, torch.float16: _lib.RZ_F16}
+_CAUSAL = {None: 0, "start": 1, "end": 2}
+_LAYOUT = {"half": 0, "interleaved": 1}
+_NORM = {"layer": 1, "rms": 2}
+
+
+class Norm(NamedTuple):
+    """A norm of rows: kind "layer" ((x - mean) / sqrt(var + eps) * weight + bias) or "rms" (x / sqrt(mean x^2 + eps) * weight + bias)."""
+    weight: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+    kind: str = "layer"
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _tokens(x, name, dim, like=None):
+    _need(isinstance(x, torch.Tensor) and x.dim() == dim, f"{name} must be a tensor of {dim} dimensions")
+    _need(x.is_cuda, f"{name} must be on the GPU (there is no CPU fallback)")
+    _need(x.dtype in _DTYPES, f"{name} must be float32, bfloat16 or float16")
+    _need(x.stride(-1) == 1 or x.shape[-1] == 1, f"{name}: columns must be contiguous")
+    _need(not (x.requires_grad and torch.is_grad_enabled()), f"{name} asks for a gradient: these operators are forward only (torch.no_grad())")
+    if like is not None:
+        _need(x.dtype == like.dtype, f"{name} must be {like.dtype}")
+        _need(x.device == like.device, f"{name} must be on {like.device}")
+
+
+def _vector(x, name, shape, device):
+    """Data pointer of a contiguous float32 tensor, None for None."""
+    if x is None:
+        return None
+    _need(isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.shape == shape, f"{name} must be float32 {tuple(shape)}")
+    _need(x.device == device and x.is_contiguous(), f"{name} must be contiguous on {device}")
+    _need(not (x.requires_grad and torch.is_grad_enabled()), f"{name} asks for a gradient: these operators are forward only (torch.no_grad())")
+    return x.data_ptr()
+
+
+def _output(out, like_shape, dtype, device, name):
+    if out is None:
+        return torch.empty(like_shape, dtype=dtype, device=device)
+    _need(isinstance(out, torch.Tensor) and out.shape == like_shape and out.dtype == dtype and out.device == device,
+          f"{name} must be {dtype} {tuple(like_shape)} on {device}")
+    _need(all(s for s, n in zip(out.stride(), out.shape) if n > 1) and (out.stride(-1) == 1 or out.shape[-1] == 1), f"{name}: columns must be contiguous, rows apart")
+    return out
+
+
+def _call(fn, device, *args):
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), fn.__name__)
+    else:                                                # kernels go to the tensors' device, on its current stream
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), fn.__name__)
+
+
+def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, axes: int = 1, scaling: Optional[dict] = None, device=None) -> Tuple[torch.Tensor, float]:
+    """(frequencies in float64, amplitude) for `rotary`: f_p = base^(-p / P), p = 0 .. P - 1, with P = rotary_dim / (2 axes) pairs per axis;
+    shape (P,) for one axis, (axes, P) for several (an image's rows and columns).
+
+    scaling stretches a table made for `original_length` positions to `factor` times as many:
+      {"kind": "linear", "factor": s}   every frequency divided by s
+      {"kind": "ntk", "factor": s}      base s^(P / (P - 1)): the fastest pair stays, the slowest is divided by s
+      {"kind": "yarn", "factor": s, "original_length": L, "beta_fast": 32, "beta_slow": 1}
+            f (g + (1 - g) / s) with g = 1 for pairs that turn at least beta_fast times over L, 0 below beta_slow, linear between; amplitude 0.1 ln s + 1
+    """
+    _need(axes >= 1 and rotary_dim >= 2 * axes and rotary_dim % (2 * axes) == 0, "rotary_dim must be a multiple of 2 * axes")
+    pairs = rotary_dim // (2 * axes)
+    p = torch.arange(pairs, dtype=torch.float64)
+    amplitude = 1.0
+    freqs = base ** (-p / pairs)
+    if scaling is not None:
+        kind, s = scaling.get("kind"), float(scaling.get("factor", 0.0))
+        _need(s >= 1.0, "scaling: factor must be at least 1")
+        if kind == "linear":
+            freqs = freqs / s
+        elif kind == "ntk":
+            _need(pairs > 1, "scaling: ntk needs more than one pair per axis")
+            freqs = (base * s ** (pairs / (pairs - 1))) ** (-p / pairs)
+        elif kind == "yarn":
+            length = float(scaling.get("original_length", 0.0))
+            fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+            _need(length > 0 and fast > slow, "scaling: yarn needs original_length > 0 and beta_fast > beta_slow")
+            g = ((freqs * length / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+            freqs = freqs * (g + (1 - g) / s)
+            amplitude = 0.1 * math.log(s) + 1.0
+        else:
+            raise ValueError("scaling: kind must be linear, ntk or yarn")
+    if axes > 1:
+        freqs = freqs.expand(axes, pairs).contiguous()
+    return freqs.to(device), amplitude
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torch.Tensor, freqs: torch.Tensor, layout: str = "half",
+           amplitude: float = 1.0, out=None):
+    """Rotary positions on q (batch, tokens, heads, head_dim) and, in the same launch, k (batch, tokens, k_heads, head_dim).
+
+    freqs: float64, (P,) or (axes, P) as `rotary_frequencies` makes them; the first 2 * freqs.numel() columns turn, the others pass through.
+    positions: int64, (tokens,) or (batch, tokens), with a last dimension of `axes` if freqs has two dimensions; |position| < 2^31.
+    layout: "half" pairs column p with p + rotary_dim / 2, "interleaved" 2 p with 2 p + 1.
+    out: tensors to write (q_out, or (q_out, k_out)); the inputs themselves are fine.  Returns q_out, or (q_out, k_out) with k."""
+    _tokens(q, "q", 4)
+    b, n, hq, d = q.shape
+    dev = q.device
+    hk = 0
+    if k is not None:
+        _tokens(k, "k", 4, q)
+        hk = k.shape[2]
+        _need(k.shape[0] == b and k.shape[1] == n and k.shape[3] == d, "q and k must agree in batch, tokens and head_dim")
+    _need(layout in _LAYOUT, "layout must be half or interleaved")
+    _need(isinstance(freqs, torch.Tensor) and freqs.dtype == torch.float64 and freqs.dim() in (1, 2) and freqs.device == dev and freqs.is_contiguous(),
+          f"freqs must be contiguous float64 (pairs,) or (axes, pairs) on {dev}")
+    axes = freqs.shape[0] if freqs.dim() == 2 else 1
+    pos = positions
+    _need(isinstance(pos, torch.Tensor) and pos.dtype == torch.int64 and pos.device == dev, f"positions must be int64 on {dev}")
+    if freqs.dim() == 2:
+        _need(pos.dim() in (2, 3) and pos.shape[-1] == axes and (pos.stride(-1) == 1 or axes == 1), "positions need a contiguous last dimension of one value per axis")
+        shape, strides = pos.shape[:-1], pos.stride()[:-1]
+    else:
+        shape, strides = pos.shape, pos.stride()
+    _need(tuple(shape) in ((n,), (b, n)), "positions must be (tokens,) or (batch, tokens)")
+    if out is None:
+        qo = torch.empty((b, n, hq, d), dtype=q.dtype, device=dev)
+        ko = torch.empty((b, n, hk, d), dtype=q.dtype, device=dev) if k is not None else None
+    else:
+        qo, ko = (out, None) if k is None else out
+        qo = _output(qo, q.shape, q.dtype, dev, "out")
+        ko = None if k is None else _output(ko, k.shape, q.dtype, dev, "out")
+    if hk:
+        ks, kos, kp, kop = k.stride(), ko.stride(), k.data_ptr(), ko.data_ptr()
+    else:
+        ks = kos = (0, 0, 0)
+        kp = kop = None
+    qs, qos = q.stride(), qo.stride()
+    a = _lib.RzRotaryArgs(_DTYPES[q.dtype], _LAYOUT[layout], b, n, hq, hk, d, 2 * freqs.numel(), axes, amplitude, q.data_ptr(), qs[0], qs[1], qs[2],
+                          kp, ks[0], ks[1], ks[2], qo.data_ptr(), qos[0], qos[1], qos[2], kop, kos[0], kos[1], kos[2],
+                          pos.data_ptr(), strides[0] if len(shape) == 2 else 0, strides[-1], freqs.data_ptr())
+    _call(_lib.load().rz_rotary, dev, ctypes.byref(a))
+    return qo if k is None else (qo, ko)
+
+
+def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk: torch.Tensor, *, lambda_init: float, scale: Optional[float] = None,
+                   causal: Optional[str] = None, kv_lens: Optional[torch.Tensor] = None, attention_mask: Optional[torch.Tensor] = None,
+                   norm_weight: Optional[torch.Tensor] = None, norm_eps: float = 1e-5, out_scale: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out_scale * norm((softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v), lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init.
+
+    q (batch, n_q, heads, 2 d), k and v (batch, n_k, kv_heads, 2 d), d = 32, 64 or 128; a row of q and k is [first map | second map]; heads a multiple
+    of kv_heads.  lambda_qk float32 (4, d) = lq1, lk1, lq2, lk2, or (heads, 4, d).  scale: 1 / sqrt(d) by default.
+    causal: "start" = query i is token i and sees keys 0 .. i; "end" = the queries are the last n_q tokens of their sequence.
+    kv_lens integer (batch,): only the first kv_lens[b] keys count.  attention_mask (batch, n_k): 0 = hidden, as a tokenizer gives it.  A query that sees
+    no key gets zeros; what hidden keys hold changes nothing.  norm_weight float32 (2 d): root-mean-square norm of every head's output.
+    16-byte alignment of q, k, v and out and of their strides is required.  Returns (batch, n_q, heads, 2 d), in `out` (no input's memory) if given."""
+    _tokens(q, "q", 4)
+    _tokens(k, "k", 4, q)
+    _tokens(v, "v", 4, q)
+    b, n_q, h, w = q.shape
+    n_k, hk = k.shape[1], k.shape[2]
+    dev = q.device
+    d = w // 2
+    _need(w in (64, 128, 256), "the last dimension must be 64, 128 or 256 (two maps of 32, 64 or 128)")
+    _need(k.shape == v.shape and k.shape[0] == b and k.shape[3] == w, "k and v must be (batch, n_k, kv_heads, 2 d), like q in batch and 2 d")
+    _need(h >= 1 and hk >= 1, "there must be a head of q and of k")
+    _need(causal in _CAUSAL, "causal must be None, start or end")
+    per_head = isinstance(lambda_qk, torch.Tensor) and lambda_qk.dim() == 3
+    lam = _vector(lambda_qk, "lambda_qk", (h, 4, d) if per_head else (4, d), dev)
+    _need(lam is not None, "lambda_qk must be a tensor")
+    if kv_lens is not None:
+        _need(isinstance(kv_lens, torch.Tensor) and kv_lens.shape == (b,) and kv_lens.device == dev and kv_lens.dtype in (torch.int32, torch.int64),
+              f"kv_lens must be int32 or int64 (batch,) on {dev}")
+        if kv_lens.dtype == torch.int64:
+            kv_lens = kv_lens.clamp(0, n_k).to(torch.int32)
+        kv_lens = kv_lens.contiguous()
+    mask = attention_mask
+    if mask is not None:
+        _need(isinstance(mask, torch.Tensor) and mask.shape == (b, n_k) and mask.device == dev and not mask.dtype.is_floating_point and not mask.dtype.is_complex,
+              f"attention_mask must be integer or bool (batch, n_k) on {dev}")
+        mask = mask.to(torch.int64)
+        if n_k > 1 and mask.stride(1) != 1:
+            mask = mask.contiguous()
+    out = _output(out, q.shape, q.dtype, dev, "out")
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    a = _lib.RzDiffAttentionArgs(_DTYPES[q.dtype], b, h, hk, n_q, n_k, d, _CAUSAL[causal], d ** -0.5 if scale is None else scale, lambda_init, norm_eps, out_scale,
+                                 q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+                                 out.data_ptr(), os[0], os[1], os[2], lam, 4 * d if per_head else 0, _vector(norm_weight, "norm_weight", (w,), dev),
+                                 None if kv_lens is None else kv_lens.data_ptr(), None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0))
+    lib, ref = _lib.load(), ctypes.byref(a)
+    need = lib.rz_diff_attention_workspace(ref)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(lib.rz_diff_attention, dev, ref, None if ws is None else ws.data_ptr(), need)
+    return out
+
+
+def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, pre_norm: Optional[Norm], post_norm: Optional[Norm] = None,
+                  scale: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, alpha: float = 1.0, dtype: Optional[torch.dtype] = None, out=None):
+    """(r, x) with r = alpha * residual + scale * gate * post_norm(y) and x = pre_norm(r): a block's output joins the residual stream and the next block's
+    operand leaves with it.
+
+    residual (rows, dim) or (batch, rows, dim), float32 or y's type; y of the same shape (None: r = alpha * residual).  scale float32 (dim,).
+    gate float32: (dim,), (batch, dim), (batch, rows, dim) or, for a residual of two dimensions, (dim,) or (rows, dim).
+    x has y's type (without y: `dtype`, else the residual's).  pre_norm None: x is None.  out: (r, x) to write; r may be `residual`, x may be `y`.
+    pre_norm's statistics are those of r in float32, before it is rounded to the residual's type."""
+    nd = residual.dim() if isinstance(residual, torch.Tensor) else 0
+    _need(nd in (2, 3), "residual must be (rows, dim) or (batch, rows, dim)")
+    _tokens(residual, "residual", nd)
+    dev, shape, dim = residual.device, residual.shape, residual.shape[-1]
+    t = dtype if dtype is not None else residual.dtype
+    if y is not None:
+        _tokens(y, "y", nd)
+        _need(y.shape == shape and y.device == dev, "y must have the residual's shape and device")
+        _need(dtype is None or dtype == y.dtype, "x has y's type")
+        t = y.dtype
+    _need(t in _DTYPES and (residual.dtype == torch.float32 or residual.dtype == t), "the residual must be float32 or of x's type")
+    _need(y is not None or (post_norm is None and scale is None and gate is None), "post_norm, scale and gate need y")
+    gs = (0, 0)
+    if gate is not None:
+        _need(isinstance(gate, torch.Tensor) and gate.dtype == torch.float32 and gate.device == dev and 1 <= gate.dim() <= nd, f"gate must be float32 on {dev}")
+        full = (dim,) if gate.dim() == 1 else shape if gate.dim() == nd else (shape[0], dim)
+        _need(tuple(gate.shape) == tuple(full) and (gate.stride(-1) == 1 or dim == 1), "gate must be (dim,), (batch, dim) or the residual's shape, columns contiguous")
+        _need(not (gate.requires_grad and torch.is_grad_enabled()), "gate asks for a gradient: these operators are forward only (torch.no_grad())")
+        st = gate.stride()
+        gs = (0, 0) if gate.dim() == 1 else (st[0], st[1]) if gate.dim() == 3 else (st[0], 0) if nd == 3 else (0, st[0])
+    ro, xo = (None, None) if out is None else out
+    write_r = y is not None or alpha != 1.0 or ro is not None or pre_norm is None
+    ro = _output(ro, shape, residual.dtype, dev, "out[0]") if write_r else residual
+    _need(xo is None or pre_norm is not None, "out[1] needs pre_norm")
+    xo = _output(xo, shape, t, dev, "out[1]") if pre_norm is not None else None
+
+    def rows(x):
+        if x is None:
+            return 0, 0
+        st = x.stride()
+        return (st[0], st[1]) if nd == 3 else (0, st[0])
+
+    def norm(x, name):
+        if x is None:
+            return 0, 0.0, None, None
+        _need(x.kind in _NORM, f"{name}.kind must be layer or rms")
+        return _NORM[x.kind], x.eps, _vector(x.weight, f"{name}.weight", (dim,), dev), _vector(x.bias, f"{name}.bias", (dim,), dev)
+
+    post, pre = norm(post_norm, "post_norm"), norm(pre_norm, "pre_norm")
+    a = _lib.RzResidualNormArgs(_DTYPES[t], _DTYPES[residual.dtype], shape[0] if nd == 3 else 1, shape[-2], dim, post[0], pre[0], alpha, post[1], pre[1],
+                                None if y is None else y.data_ptr(), *rows(y), residual.data_ptr(), *rows(residual),
+                                ro.data_ptr() if write_r else None, *rows(ro), None if xo is None else xo.data_ptr(), *rows(xo),
+                                post[2], post[3], _vector(scale, "scale", (dim,), dev), None if gate is None else gate.data_ptr(), *gs, pre[2], pre[3])
+    _call(_lib.load().rz_residual_norm, dev, ctypes.byref(a))
+    return ro, xo

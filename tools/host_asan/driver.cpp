@@ -116,6 +116,52 @@ int main(int argc, char** argv) {
         OK(rz_vision_forward(h, px.data(), 1, 3, 224, 224, nullptr, nullptr));
         float ms[8]; int64_t launches[8];
         OK(rz_profile_read(h, ms, launches));
+        // a differential-attention block on strided views of exact buffers, and its refusals
+        const size_t es = dt == 0 ? 4 : 2;
+        const int b = 2, n = 5, d = 32, hq = 4, hk = 2, row = (hq + 2 * hk) * 2 * d;
+        std::vector<unsigned char> qkv((size_t)b * n * row * es), att((size_t)b * n * hq * 2 * d * es), xn(att.size());
+        std::vector<float> res((size_t)b * n * hq * 2 * d), lam(4 * d), w(hq * 2 * d, 1.f), gate((size_t)b * hq * 2 * d, 1.f);
+        std::vector<int64_t> pos((size_t)b * n * 2, 3), keys_seen((size_t)b * n, 1);
+        std::vector<double> freqs(d, 0.1);
+        std::vector<int32_t> lens(b, n);
+        rz_rotary_args ra = {};
+        ra.dtype = dt; ra.batch = b; ra.tokens = n; ra.q_heads = hq; ra.k_heads = hk; ra.head_dim = 2 * d; ra.rotary_dim = 2 * d; ra.n_axes = 2; ra.amplitude = 1.f;
+        ra.q_dev = qkv.data(); ra.k_dev = qkv.data() + (size_t)hq * 2 * d * es; ra.q_out_dev = (void*)ra.q_dev; ra.k_out_dev = (void*)ra.k_dev;
+        ra.q_batch_stride = ra.k_batch_stride = ra.q_out_batch_stride = ra.k_out_batch_stride = (int64_t)n * row;
+        ra.q_token_stride = ra.k_token_stride = ra.q_out_token_stride = ra.k_out_token_stride = row;
+        ra.q_head_stride = ra.k_head_stride = ra.q_out_head_stride = ra.k_out_head_stride = 2 * d;
+        ra.positions_dev = pos.data(); ra.positions_batch_stride = 2 * n; ra.positions_token_stride = 2; ra.freqs_dev = freqs.data();
+        OK(rz_rotary(&ra, nullptr));
+        FAILS(rz_rotary(nullptr, nullptr));
+        ra.rotary_dim = 2 * d + 2; FAILS(rz_rotary(&ra, nullptr));
+        ra.rotary_dim = 2 * d; ra.n_axes = 3; FAILS(rz_rotary(&ra, nullptr));
+        ra.n_axes = 1; ra.k_dev = nullptr; FAILS(rz_rotary(&ra, nullptr));
+        ra.tokens = 0; OK(rz_rotary(&ra, nullptr));
+        rz_diff_attention_args da = {};
+        da.dtype = dt; da.batch = b; da.heads = hq; da.kv_heads = hk; da.n_q = da.n_k = n; da.head_dim = d; da.scale = 0.2f; da.out_scale = 1.f;
+        da.q_dev = qkv.data(); da.k_dev = qkv.data() + (size_t)hq * 2 * d * es; da.v_dev = qkv.data() + (size_t)(hq + hk) * 2 * d * es; da.out_dev = att.data();
+        da.q_batch_stride = da.k_batch_stride = da.v_batch_stride = (int64_t)n * row; da.q_token_stride = da.k_token_stride = da.v_token_stride = row;
+        da.q_head_stride = da.k_head_stride = da.v_head_stride = da.out_head_stride = 2 * d; da.out_token_stride = hq * 2 * d; da.out_batch_stride = (int64_t)n * hq * 2 * d;
+        da.lambda_qk_dev = lam.data(); da.norm_weight_dev = w.data(); da.kv_lens_dev = lens.data(); da.mask_dev = keys_seen.data(); da.mask_batch_stride = n;
+        const size_t dws = rz_diff_attention_workspace(&da);
+        std::vector<unsigned char> attws(dws + 16);
+        OK(rz_diff_attention(&da, attws.data(), dws, nullptr));
+        da.head_dim = 48; FAILS(rz_diff_attention(&da, attws.data(), dws, nullptr));
+        if (rz_diff_attention_workspace(&da) != 0) return 6;
+        da.head_dim = d; da.kv_heads = 3; FAILS(rz_diff_attention(&da, attws.data(), dws, nullptr));
+        da.kv_heads = hk; da.q_token_stride = row + 1; FAILS(rz_diff_attention(&da, attws.data(), dws, nullptr));
+        da.q_token_stride = row; da.scale = 0.f; FAILS(rz_diff_attention(&da, attws.data(), dws, nullptr));
+        da.scale = 1.f; da.n_k = 0; da.k_dev = da.v_dev = nullptr; OK(rz_diff_attention(&da, attws.data(), dws, nullptr));
+        rz_residual_norm_args na = {};
+        na.dtype = dt; na.resid_dtype = 0; na.batch = b; na.rows = n; na.dim = hq * 2 * d; na.post_kind = 2; na.pre_kind = 1; na.alpha = 1.f;
+        na.y_dev = att.data(); na.out_dev = xn.data(); na.resid_dev = res.data(); na.resid_out_dev = res.data();
+        na.y_row_stride = na.out_row_stride = na.resid_row_stride = na.resid_out_row_stride = na.dim;
+        na.y_batch_stride = na.out_batch_stride = na.resid_batch_stride = na.resid_out_batch_stride = (int64_t)n * na.dim;
+        na.scale_dev = na.post_weight_dev = na.pre_weight_dev = w.data(); na.gate_dev = gate.data(); na.gate_batch_stride = na.dim;
+        OK(rz_residual_norm(&na, nullptr));
+        na.dim = 0; FAILS(rz_residual_norm(&na, nullptr));
+        na.dim = 16385; FAILS(rz_residual_norm(&na, nullptr));
+        na.dim = hq * 2 * d; na.y_dev = nullptr; FAILS(rz_residual_norm(&na, nullptr));
         OK(rz_destroy(h));
         printf("[host_asan] dtype %d: clean, %d kernel ranges checked so far\n", dt, rz::host_asan_ranges_checked());
     }

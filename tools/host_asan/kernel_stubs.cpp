@@ -310,6 +310,55 @@ hipError_t launch_grounding_points(const float* maps, int64_t stride, unsigned l
     return hipSuccess;
 }
 
+// ---- differential-attention block (rotary.hip, diff_attention.hip, residual_norm.hip): first and last row of every strided tensor -----
+static void rows3(void* p, int64_t sb, int64_t st, int64_t sh, int b, int t, int h, size_t cols, size_t es, bool write, const char* what) {
+    for (int i : {0, b - 1})
+        for (int j : {0, t - 1})
+            for (int k : {0, h - 1}) {
+                char* row = (char*)p + (size_t)(i * sb + j * st + k * sh) * es;
+                if (write) wr(row, cols * es, what); else rd(row, cols * es, what);
+            }
+}
+hipError_t launch_rotary(const rz_rotary_args& a, hipStream_t) {
+    const size_t es = esz(a.dtype);
+    rows3((void*)a.q_dev, a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.batch, a.tokens, a.q_heads, a.head_dim, es, false, "rotary q");
+    rows3(a.q_out_dev, a.q_out_batch_stride, a.q_out_token_stride, a.q_out_head_stride, a.batch, a.tokens, a.q_heads, a.head_dim, es, true, "rotary q out");
+    if (a.k_heads) {
+        rows3((void*)a.k_dev, a.k_batch_stride, a.k_token_stride, a.k_head_stride, a.batch, a.tokens, a.k_heads, a.head_dim, es, false, "rotary k");
+        rows3(a.k_out_dev, a.k_out_batch_stride, a.k_out_token_stride, a.k_out_head_stride, a.batch, a.tokens, a.k_heads, a.head_dim, es, true, "rotary k out");
+    }
+    rd(a.freqs_dev, (size_t)a.rotary_dim / 2 * 8, "rotary freqs");
+    rd(a.positions_dev + (a.batch - 1) * a.positions_batch_stride + (a.tokens - 1) * a.positions_token_stride, (size_t)a.n_axes * 8, "rotary positions");
+    return hipSuccess;
+}
+size_t diff_attention_workspace_bytes(const rz_diff_attention_args& a) { return a.n_k > 4096 ? (size_t)a.batch * a.heads * a.n_q * 16 : 0; }
+hipError_t launch_diff_attention(const rz_diff_attention_args& a, void* ws, hipStream_t) {
+    const size_t es = esz(a.dtype), cols = 2 * (size_t)a.head_dim;
+    rows3((void*)a.q_dev, a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.batch, a.n_q, a.heads, cols, es, false, "diff_attention q");
+    if (a.n_k) {
+        rows3((void*)a.k_dev, a.k_batch_stride, a.k_token_stride, a.k_head_stride, a.batch, a.n_k, a.kv_heads, cols, es, false, "diff_attention k");
+        rows3((void*)a.v_dev, a.v_batch_stride, a.v_token_stride, a.v_head_stride, a.batch, a.n_k, a.kv_heads, cols, es, false, "diff_attention v");
+    }
+    rows3(a.out_dev, a.out_batch_stride, a.out_token_stride, a.out_head_stride, a.batch, a.n_q, a.heads, cols, es, true, "diff_attention out");
+    rd(a.lambda_qk_dev + (a.heads - 1) * a.lambda_head_stride, (size_t)4 * a.head_dim * 4, "diff_attention lambda");
+    if (a.norm_weight_dev) rd(a.norm_weight_dev, cols * 4, "diff_attention norm");
+    if (a.kv_lens_dev) rd(a.kv_lens_dev, (size_t)a.batch * 4, "diff_attention lens");
+    if (a.mask_dev && a.n_k) rd(a.mask_dev + (a.batch - 1) * a.mask_batch_stride, (size_t)a.n_k * 8, "diff_attention mask");
+    if (const size_t n = diff_attention_workspace_bytes(a)) wr(ws, n, "diff_attention workspace");
+    return hipSuccess;
+}
+hipError_t launch_residual_norm(const rz_residual_norm_args& a, hipStream_t) {
+    const size_t es = esz(a.dtype), rs = esz(a.resid_dtype), d = a.dim;
+    if (a.y_dev) rows3((void*)a.y_dev, a.y_batch_stride, a.y_row_stride, 0, a.batch, a.rows, 1, d, es, false, "residual_norm y");
+    rows3((void*)a.resid_dev, a.resid_batch_stride, a.resid_row_stride, 0, a.batch, a.rows, 1, d, rs, false, "residual_norm residual");
+    if (a.resid_out_dev) rows3(a.resid_out_dev, a.resid_out_batch_stride, a.resid_out_row_stride, 0, a.batch, a.rows, 1, d, rs, true, "residual_norm residual out");
+    if (a.out_dev) rows3(a.out_dev, a.out_batch_stride, a.out_row_stride, 0, a.batch, a.rows, 1, d, es, true, "residual_norm out");
+    for (const float* w : {a.post_weight_dev, a.post_bias_dev, a.scale_dev, a.pre_weight_dev, a.pre_bias_dev})
+        if (w) rd(w, d * 4, "residual_norm vector");
+    if (a.gate_dev) rows3((void*)a.gate_dev, a.gate_batch_stride, a.gate_row_stride, 0, a.batch, a.rows, 1, d, 4, false, "residual_norm gate");
+    return hipSuccess;
+}
+
 // ---- preprocessing (preprocess.hip) -------------------------------------------------------------------------------------------
 struct PreDescMock { const void* img; int dtype, H, W, C; int pad_left, pad_top, PH, PW; const int* bounds_h; const int* kk_h; int ksize_h; const int* bounds_v; const int* kk_v; int ksize_v; int64_t a8, b8, c8; };
 size_t preprocess_batch_desc_bytes(int n) { return ((size_t)n * sizeof(PreDescMock) + 8 * (size_t)n + 255) / 256 * 256; }
