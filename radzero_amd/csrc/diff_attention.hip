@@ -5,7 +5,18 @@
 //   lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init
 //   out[i] = out_scale * o[i] / sqrt(mean(o[i]^2) + eps) * w      (or out_scale * o[i] without a norm weight)
 //
-// One pass over the keys: each map keeps its running maximum and sum and its own sum of values; the maps meet when both sums are known.
+// One pass over the keys: each map keeps its own reference maximum m, sum l and sum of values O, all fp32; the maps meet when both sums are known.
+//
+// A wave owns 32 query rows (query-major, the heads that share a key head beside each other, so that one tile of keys serves all of them) and computes
+// everything transposed on 32x32 MFMAs: S^T = K Q^T puts a query in a column = in a lane, so that its maximum, its sum and every rescale are
+// that lane's own; P^T then is the B operand of O^T = V^T P^T as it stands in the registers, and one fragment of V^T serves both maps.
+//   16-bit: 32x32x16, V^T fragments by transposing LDS reads;  fp32: 32x32x2 (exact), V^T fragments are plain reads of a row.
+// Two ways to share the work:
+//   rows  4 waves x 32 rows on the same key tiles (double-buffered in LDS, filled by LDS-DMA): many queries
+//   keys  4 waves on the same 32 rows, every wave its own key tiles, joined in LDS: few queries over many keys
+// Either may also split the keys over workgroups; partial (O, m, l) then go through the workspace and a second kernel joins them.
+#include <type_traits>
+
 #include "rz_common.h"
 #include "rz_kernels.h"
 
@@ -13,82 +24,635 @@ namespace rz {
 
 namespace {
 
-// one wave per query row and head; a lane owns one key of a tile of 64 for the scores, and every 64th column for the values
-template <typename T> __global__ __launch_bounds__(64) void diff_attention_kernel(const rz_diff_attention_args a) {
-    const int lane = threadIdx.x, d = a.head_dim, w = 2 * d;
-    int64_t id = blockIdx.x;
-    const int h = (int)(id % a.heads);
-    id /= a.heads;
-    const int i = (int)(id % a.n_q), b = (int)(id / a.n_q), hk = h / (a.heads / a.kv_heads);
-    const T* q = (const T*)a.q_dev + b * a.q_batch_stride + i * a.q_token_stride + h * a.q_head_stride;
-    const T* k = (const T*)a.k_dev + b * a.k_batch_stride + hk * a.k_head_stride;
-    const T* v = (const T*)a.v_dev + b * a.v_batch_stride + hk * a.v_head_stride;
-    int n = a.n_k;
-    if (a.kv_lens_dev) n = min(max(a.kv_lens_dev[b], 0), n);
-    int end = n;
-    if (a.causal) end = min(n, i + 1 + (a.causal == RZ_CAUSAL_END ? n - a.n_q : 0));
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2][4] = {};
-    const float c = a.scale * 1.44269504088896340736f;
-    for (int j0 = 0; j0 < end; j0 += 64) {
-        const int j = j0 + lane;
-        const bool seen = j < end && (!a.mask_dev || a.mask_dev[b * a.mask_batch_stride + j] != 0);
-        if (!__ballot(seen)) continue;
-        float p[2];
-        for (int x = 0; x < 2; ++x) {
-            float s = -INFINITY;
-            if (seen) {
-                s = 0.f;
-                for (int e = 0; e < d; ++e) s = fmaf(to_f32(q[x * d + e]), to_f32(k[j * a.k_token_stride + x * d + e]), s);
-            }
-            const float mn = fmaxf(m[x], wave_max(s));
-            const float f = mn == -INFINITY ? 1.f : exp2f((m[x] - mn) * c);
-            p[x] = !seen ? 0.f : mn == -INFINITY ? s * 0.f : exp2f((s - mn) * c);
-            l[x] = l[x] * f + wave_sum(p[x]);
-            for (int y = 0; y < 4; ++y) o[x][y] *= f;
-            m[x] = mn;
-        }
-        for (int t = 0; t < 64; ++t) {
-            if (!__shfl((int)seen, t, 64)) continue;
-            const float p1 = __shfl(p[0], t, 64), p2 = __shfl(p[1], t, 64);
-            for (int y = 0; y < 4 && lane + 64 * y < w; ++y) {
-                const float x = to_f32(v[(j0 + t) * a.v_token_stride + lane + 64 * y]);
-                o[0][y] = fmaf(p1, x, o[0][y]);
-                o[1][y] = fmaf(p2, x, o[1][y]);
-            }
-        }
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// 16-byte operand chunk: 8 elements of K per 32x32x16 step, or 4 of them as four 32x32x2 steps
+template <typename T> struct Op;
+template <> struct Op<bf16_t> {
+    typedef bf16x8 chunk;
+    static __device__ __forceinline__ f32x16 mma(chunk a, chunk b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Op<f16_t> {
+    typedef f16x8 chunk;
+    static __device__ __forceinline__ f32x16 mma(chunk a, chunk b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Op<float> {
+    typedef f32x4 chunk;
+    static __device__ __forceinline__ f32x16 mma(chunk a, chunk b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
     }
-    const float* lam = a.lambda_qk_dev + h * a.lambda_head_stride;
+};
+
+// the larger of a lane and the lane 32 away, the sum of the two (both hold the same query)
+__device__ __forceinline__ float pair_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename T, int D> struct Shape {
+    static constexpr int RB = 2 * D * (int)sizeof(T);          // bytes of a key's row: both maps' halves; the same for its values
+    static constexpr int CH = RB / 16;                         // 16-byte chunks of a row
+    static constexpr int NT = D * (int)sizeof(T) / 32;         // 32-byte steps of a score product
+    static constexpr int NC = 2 * D / 32;                      // 32-column blocks of the values
+    // LDS images: chunk c of row r stands at c ^ swz(r).  Scores read 32 rows x one chunk, 16 different rows must not meet in a bank (256 bytes):
+    // with 128-byte rows two of them share the banks.  Transposing reads take 4 rows x 64 bytes at a time, fp32 reads 2 rows 4 apart x 128 bytes.
+    static __device__ __forceinline__ int swz_k(int r) { return RB == 128 ? (r >> 1) & 7 : r & 15; }
+    static __device__ __forceinline__ int swz_v(int r) {
+        if constexpr (sizeof(T) == 4) return ((r >> 2) & 1) << 3;
+        else return RB == 128 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+    }
+};
+
+constexpr int kRowsWaves = 4;
+// keys of a tile: 64 where the tile buffers of two workgroups fit the LDS, 32 for long rows
+template <typename T, int D> constexpr int rows_tile() { return Shape<T, D>::RB <= 256 ? 64 : 32; }
+// waves that split the keys of the same rows: as many private double buffers of 32 keys as 128 KB hold
+template <typename T, int D> constexpr int keys_waves() { return Shape<T, D>::RB <= 256 ? 4 : Shape<T, D>::RB == 512 ? 2 : 1; }
+
+struct Plan { int keys_mode, splits; };
+
+struct Args {
+    rz_diff_attention_args a;
+    int group, rows, row_blocks, splits;                       // heads per key head, query rows per key head, their blocks, key splits
+    float* ws;
+};
+
+// partial results of a split, floats: [batch][kv head][split][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
+__host__ __device__ inline int64_t part_rows(const Args& x) { return (int64_t)x.a.batch * x.a.kv_heads * x.splits * x.rows; }
+
+// lambda of query head h, by the whole wave
+__device__ __forceinline__ float head_lambda(const rz_diff_attention_args& a, int h, int lane) {
+    const float* p = a.lambda_qk_dev + (int64_t)h * a.lambda_head_stride;
+    const int d = a.head_dim;
     float x1 = 0.f, x2 = 0.f;
     for (int e = lane; e < d; e += 64) {
-        x1 = fmaf(lam[e], lam[d + e], x1);
-        x2 = fmaf(lam[2 * d + e], lam[3 * d + e], x2);
+        x1 = fmaf(p[e], p[d + e], x1);
+        x2 = fmaf(p[2 * d + e], p[3 * d + e], x2);
     }
-    const float lambda = expf(wave_sum(x1)) - expf(wave_sum(x2)) + a.lambda_init;
-    const float r1 = l[0] == 0.f ? 0.f : 1.f / l[0], r2 = l[1] == 0.f ? 0.f : lambda / l[1];
+    return expf(wave_sum(x1)) - expf(wave_sum(x2)) + a.lambda_init;
+}
+
+// ---- one wave's 32 query rows ---------------------------------------------------------------------------------------------------
+template <typename T, int D> struct Wave {
+    typedef Shape<T, D> S;
+    typedef typename Op<T>::chunk chunk;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    static constexpr int NT = S::NT, NC = S::NC, RB = S::RB;
+
+    chunk q[2][NT];
+    f32x16 o[2][NC];
+    float m[2], mc[2], l[2];          // reference maximum (raw score), the same times c, this lane's share of the sum
+    float c;                          // scale * log2(e)
+    int lane, h;                      // h: which half of every 8 keys the lane holds
+    bool started;                     // every row has a reference maximum (wave-uniform)
+
+    __device__ __forceinline__ void init(const Args& x, const T* qrow) {
+        c = x.a.scale * 1.44269504088896340736f;
+        started = false;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            m[y] = -INFINITY, mc[y] = 0.f, l[y] = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) q[y][t] = *reinterpret_cast<const chunk*>((const char*)qrow + (y * NT + t) * 32 + h * 16);
+#pragma unroll
+            for (int cb = 0; cb < NC; ++cb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[y][cb][e] = 0.f;
+        }
+    }
+
+    // S^T of 32 keys: register e is key 8 (e / 4) + 4 h + e % 4 of them
+    __device__ __forceinline__ f32x16 scores(const char* kt, int y) const {
+        f32x16 s = {};
+        const int r = lane & 31;
+        const char* row = kt + r * RB;
+        const int x = S::swz_k(r);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s = Op<T>::mma(*reinterpret_cast<const chunk*>(row + (((y * NT + t) * 2 + h) ^ x) * 16), q[y][t], s);
+        return s;
+    }
+
+    // a first tile, a tile with hidden keys, or one whose weights outgrew the reference: the maximum is taken, O and l follow it
+    __device__ __forceinline__ void recentre(f32x16& s, int y, uint32_t seen) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[e] = (seen >> (8 * (e / 4) + e % 4)) & 1 ? s[e] : -INFINITY;
+            mx = fmaxf(mx, s[e]);
+        }
+        const float mn = fmaxf(m[y], pair_max(mx));
+        if (__any(mn > m[y])) {
+            const float mcn = mn == -INFINITY ? 0.f : mn * c, f = m[y] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc[y] - mcn);      // m == mn: 1
+            l[y] *= f;
+#pragma unroll
+            for (int cb = 0; cb < NC; ++cb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[y][cb][e] *= f;
+            m[y] = mn;
+            mc[y] = mcn;
+        }
+    }
+
+    __device__ __forceinline__ float weights(f32x16& s, int y) const {
+        float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -mc[y]));
+            s[e + 1] = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c, -mc[y]));
+            t0 += s[e];
+            t1 += s[e + 1];
+        }
+        return t0 + t1;
+    }
+
+    // O^T += V^T P^T for both maps
+    __device__ __forceinline__ void values(const char* vt, const f32x16 (&p)[2]) {
+        if constexpr (sizeof(T) == 4) {
+            const int col = lane & 31;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = 8 * (e / 4) + 4 * h + e % 4;
+#pragma unroll
+                for (int cb = 0; cb < NC; ++cb) {
+                    const float v = *reinterpret_cast<const float*>(vt + r * RB + (((cb * 8 + (col >> 2)) ^ S::swz_v(r)) << 4) + (col & 3) * 4);
+                    o[0][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[0][e], o[0][cb], 0, 0, 0);
+                    o[1][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[1][e], o[1][cb], 0, 0, 0);
+                }
+            }
+        } else {
+            chunk w[2][2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    w[y][u] = pack8<T>(p[y][8 * u], p[y][8 * u + 1], p[y][8 * u + 2], p[y][8 * u + 3], p[y][8 * u + 4], p[y][8 * u + 5], p[y][8 * u + 6], p[y][8 * u + 7]);
+            // a transposing read gives lane x of 16 column x of 4 rows; the lanes of a group point at those rows, 4 lanes (32 bytes) each
+            const int x = lane & 15, sub = (lane >> 4) & 1, r0 = 4 * h + (x >> 2), swz = S::swz_v(x >> 2);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int cb = 0; cb < NC; ++cb) {
+                    const char* at = vt + r0 * RB + (((cb * 4 + sub * 2 + ((x & 3) >> 1)) ^ swz) << 4) + (x & 1) * 8;
+                    const s16x4 a = tr(at + (16 * u) * RB), b = tr(at + (16 * u + 8) * RB);
+                    const chunk v = __builtin_bit_cast(chunk, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[0][cb] = Op<T>::mma(v, w[0][u], o[0][cb]);
+                    o[1][cb] = Op<T>::mma(v, w[1][u], o[1][cb]);
+                }
+        }
+    }
+    static __device__ __forceinline__ s16x4 tr(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p); }
+
+    // 32 keys that stand in LDS at kt, vt.  seen: bit j = this lane's query sees key j; all: every query of the wave sees every key;
+    // odd: bit j = key j's values were not all finite (take_odd)
+    __device__ __forceinline__ void block(const char* kt, const char* vt, uint32_t seen, bool all, uint32_t odd) {
+        f32x16 s[2];
+        float t[2];
+        bool fine = false;
+        if (all && started) {
+            // No maximum here: a weight that outgrows the reference shows in the sum.  2^15 keeps every weight below the largest f16.
+            s[0] = scores(kt, 0);
+            s[1] = scores(kt, 1);
+            t[0] = weights(s[0], 0);
+            t[1] = weights(s[1], 1);
+            fine = !__any(!(t[0] <= 32768.f && t[1] <= 32768.f));
+        }
+        if (!fine) {
+            // Hardly ever taken: one map after the other, on fragments read anew.  What the path above holds is not kept for this one (registers).
+            const uint32_t mine = seen >> (4 * h);
+            int zero = 0;
+            asm("" : "+v"(zero));
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                __builtin_amdgcn_sched_barrier(0);
+                s[y] = scores(kt + zero, y);
+                recentre(s[y], y, mine);
+                t[y] = weights(s[y], y);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            started = __all(m[0] > -INFINITY && m[1] > -INFINITY);
+        }
+        const float poison = seen & odd ? __builtin_nanf("") : 0.f;
+        l[0] += t[0] + poison;
+        l[1] += t[1];
+        values(vt, s);
+    }
+};
+
+// bits of the keys below `n` (any n)
+__device__ __forceinline__ uint64_t below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
+// Fills LDS rows [0, ROWS) x RB bytes with keys j0 ..; wave w of W.  Keys that nobody may see (bits 0: hidden, or behind the last) are replaced by the first that
+// somebody does: their weights are 0, and 0 * (what a hidden place holds) would not be.
+template <typename T, int D, int ROWS, int W, bool VALUES>
+__device__ __forceinline__ void stage(char* lds, const char* src, int64_t stride, int j0, uint64_t bits, int w, int lane) {
+    typedef Shape<T, D> S;
+    constexpr int per = 1024 / S::RB, N = ROWS * S::RB / 1024 / W;         // rows of one LDS-DMA instruction (1 KB), instructions of a wave
+    static_assert(S::RB <= 1024 && ROWS * S::RB % (1024 * W) == 0, "tile and waves do not fit");
+    const int sub = lane / S::CH, cp = lane % S::CH;
+    const int first = __builtin_ctzll(bits);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r0 = (w * N + i) * per, r = r0 + sub;
+        const int key = j0 + ((bits >> r) & 1 ? r : first);
+        const char* p = src + (int64_t)key * stride + ((cp ^ (VALUES ? S::swz_v(r) : S::swz_k(r))) << 4);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)(lds + r0 * S::RB), 16, 0, 0);
+    }
+}
+
+// Values that are not finite, in a tile that not every query sees in full (causal): 0 * inf is not 0, so they would reach queries that must not see them.
+// Returns the keys (bits) that hold any; take_odd then clears those values in LDS, and a query that does see such a key becomes NaN through its sum.
+template <typename T> __device__ __forceinline__ bool odd_chunk(const u32x4& v) {
+    constexpr uint32_t exponent = std::is_same<T, float>::value ? 0x7f800000u : std::is_same<T, bf16_t>::value ? 0x7f807f80u : 0x7c007c00u;
+    constexpr uint32_t one = std::is_same<T, float>::value ? 0x00800000u : std::is_same<T, bf16_t>::value ? 0x00800080u : 0x04000400u;
+    uint32_t t = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t |= (v[e] & exponent) + one;              // an exponent of ones carries into the sign's place
+    return t & (std::is_same<T, float>::value ? 0x80000000u : 0x80008000u);
+}
+template <typename T, int D, int ROWS> __device__ __forceinline__ uint64_t odd_keys(const char* vt, int lane) {
+    typedef Shape<T, D> S;
+    constexpr int N = ROWS * S::RB / 1024, per = 64 / S::CH;
+    bool any = false;
+    for (int n = 0; n < N; ++n) any |= odd_chunk<T>(*reinterpret_cast<const u32x4*>(vt + (n * 64 + lane) * 16));
+    uint64_t keys = 0;
+    if (__any(any))
+        for (int n = 0; n < N; ++n) {
+            const uint64_t b = __ballot(odd_chunk<T>(*reinterpret_cast<const u32x4*>(vt + (n * 64 + lane) * 16)));
+            for (int r = 0; r < per; ++r)
+                if (b >> (r * S::CH) & (S::CH == 64 ? ~0ull : (1ull << (S::CH & 63)) - 1)) keys |= 1ull << (n * per + r);
+        }
+    return keys;
+}
+template <typename T, int D, int ROWS> __device__ __forceinline__ void take_odd(char* vt, int lane) {
+    constexpr int N = ROWS * Shape<T, D>::RB / (64 * (int)sizeof(T));
+    for (int n = 0; n < N; ++n) {
+        T* v = (T*)vt + n * 64 + lane;
+        if (!(fabsf(to_f32(*v)) < INFINITY)) *v = (T)0.f;
+    }
+}
+
+template <typename T, int D> struct Out {
+    typedef Shape<T, D> S;
+    // writes column blocks cb = first, first + step, ... of a finished row: 4 columns per 4 registers; `ss`: this lane's share of the sum of squares
+    template <int STEP, int COUNT>
+    static __device__ __forceinline__ void store(const Args& x, const f32x16 (&o)[COUNT], int first, int b, int i, int head, bool live, float factor, int h) {
+        if (!live) return;
+        T* out = (T*)x.a.out_dev + b * x.a.out_batch_stride + i * x.a.out_token_stride + head * x.a.out_head_stride;
+#pragma unroll
+        for (int n = 0; n < COUNT; ++n) {
+            const int cb = first + n * STEP;
+            if (cb >= S::NC) break;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = cb * 32 + 8 * g + 4 * h;
+                f32x4 w = {factor, factor, factor, factor};
+                if (x.a.norm_weight_dev) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] *= x.a.norm_weight_dev[col + e];
+                }
+                *reinterpret_cast<typename Traits<T>::vec4*>(out + col) = pack4<T>(o[n][4 * g] * w[0], o[n][4 * g + 1] * w[1], o[n][4 * g + 2] * w[2], o[n][4 * g + 3] * w[3]);
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, float sum_of_squares) {
+    return a.norm_weight_dev ? a.out_scale / sqrtf(sum_of_squares / (float)(2 * a.head_dim) + a.norm_eps) : a.out_scale;
+}
+
+// What a workgroup works on, from its id: row blocks innermost (they read the same keys), then splits, then key heads
+struct Work {
+    int rb, split, hk, b;
+    __device__ __forceinline__ Work(const Args& x) {
+        int id = xcd_remap(blockIdx.x, gridDim.x);
+        rb = x.row_blocks - 1 - id % x.row_blocks;                         // causal: the longest first
+        id /= x.row_blocks;
+        split = id % x.splits;
+        id /= x.splits;
+        hk = id % x.a.kv_heads;
+        b = id / x.a.kv_heads;
+    }
+};
+
+template <typename T, int D, bool KEYS, int MINW = (sizeof(T) == 2 && D <= 64 ? 2 : 1)>
+__global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW) void diff_attention_kernel(const Args x) {
+    typedef Shape<T, D> S;
+    constexpr int W = KEYS ? keys_waves<T, D>() : kRowsWaves, BN = KEYS ? 32 : rows_tile<T, D>(), TILE = BN * S::RB, NC = S::NC;
+    constexpr int BUF = 2 * TILE;                                          // keys, then values
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const rz_diff_attention_args& a = x.a;
+    const Work at(x);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row0 = at.rb * (KEYS ? 32 : 32 * W) + (KEYS ? 0 : 32 * wave), row = row0 + (lane & 31);
+    const bool live = row < x.rows;
+    const int rr = min(row, x.rows - 1), i = rr / x.group, head = at.hk * x.group + rr % x.group;
+
+    int n = a.n_k;
+    if (a.kv_lens_dev) n = min(max(a.kv_lens_dev[at.b], 0), n);
+    const int shift = a.causal == RZ_CAUSAL_END ? n - a.n_q : 0;
+    auto limit = [&](int query) { return a.causal ? min(n, query + 1 + shift) : n; };       // keys that a query may see at most (may be negative)
+    const int lim = limit(i);
+    const int last = min(at.rb * (KEYS ? 32 : 32 * W) + (KEYS ? 32 : 32 * W), x.rows) - 1;
+    const int end = max(limit(last / x.group), 0);                         // of the workgroup
+    const int wave_first = limit(min(row0, x.rows - 1) / x.group);         // keys that every query of the wave sees, but for hidden ones
+    const int group_first = limit(at.rb * (KEYS ? 32 : 32 * W) / x.group); // the same of the workgroup
+    int begin = 0, stop = end;
+    if (x.splits > 1) {
+        const int per = ((end + x.splits - 1) / x.splits + 63) / 64 * 64;
+        begin = min(at.split * per, end);
+        stop = min(begin + per, end);
+    }
+
+    Wave<T, D> wv;
+    wv.lane = lane;
+    wv.h = lane >> 5;
+    wv.init(x, (const T*)a.q_dev + at.b * a.q_batch_stride + i * a.q_token_stride + head * a.q_head_stride);
+
+    const char* kp = (const char*)((const T*)a.k_dev + at.b * a.k_batch_stride + at.hk * a.k_head_stride);
+    const char* vp = (const char*)((const T*)a.v_dev + at.b * a.v_batch_stride + at.hk * a.v_head_stride);
+    const int64_t ks = a.k_token_stride * (int64_t)sizeof(T), vs = a.v_token_stride * (int64_t)sizeof(T);
+    const int64_t* mask = a.mask_dev ? a.mask_dev + at.b * a.mask_batch_stride : nullptr;
+    constexpr int STEP = KEYS ? BN * W : BN;
+    const int j_first = begin + (KEYS ? wave * BN : 0);
+    // keys of the tile at j that some query may see; the mask's values are asked for one tile ahead
+    auto ask = [&](int j) -> int64_t { return mask && j + lane < stop && lane < BN ? mask[j + lane] : 0; };
+    auto answer = [&](int j, int64_t v) -> uint64_t {
+        const uint64_t in = below(min(stop - j, BN));
+        return mask ? in & __ballot(v != 0) : in;
+    };
+    auto fill = [&](char* buf, int j, uint64_t bits) {
+        stage<T, D, BN, KEYS ? 1 : W, false>(buf, kp, ks, j, bits, KEYS ? 0 : wave, lane);
+        stage<T, D, BN, KEYS ? 1 : W, true>(buf + TILE, vp, vs, j, bits, KEYS ? 0 : wave, lane);
+    };
+    char* mine = lds + (KEYS ? wave * 2 * BUF : 0);
+    // the next tile with a key that somebody sees
+    int j_next = j_first;
+    uint64_t bits_next = answer(j_next, ask(j_next));
+    int64_t asked = ask(j_next + STEP);
+    auto skip_empty = [&] {
+        while (!bits_next && j_next < stop) {
+            j_next += STEP;
+            bits_next = answer(j_next, asked);
+            asked = ask(j_next + STEP);
+        }
+    };
+    skip_empty();
+    if (bits_next) fill(mine, j_next, bits_next);
+    int turn = 0;
+    while (bits_next) {
+        const int j = j_next;
+        const uint64_t bits = bits_next;
+        // everything asked for so far has landed; the other buffer's readers are done
+        if constexpr (KEYS) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else __syncthreads();
+        j_next = j + STEP;
+        bits_next = answer(j_next, asked);
+        asked = ask(j_next + STEP);
+        skip_empty();
+        if (bits_next) fill(mine + (turn ^ 1) * BUF, j_next, bits_next);
+        char* buf = mine + turn * BUF;
+        const bool all = bits == below(BN) && j + BN <= wave_first;
+        uint64_t odd = 0;
+        if (a.causal && j + BN > group_first) {                            // the same for all waves that share the tile
+            odd = odd_keys<T, D, BN>(buf + TILE, lane);
+            if (odd) {
+                if constexpr (!KEYS) __syncthreads();
+                take_odd<T, D, BN>(buf + TILE, lane);
+                if constexpr (KEYS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                else __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int kb = 0; kb < BN / 32; ++kb) {
+            const uint32_t seen = (uint32_t)((bits & below(lim - j)) >> (32 * kb));
+            wv.block(buf + kb * 32 * S::RB, buf + TILE + kb * 32 * S::RB, seen, all, (uint32_t)(odd >> (32 * kb)));
+        }
+        turn ^= 1;
+    }
+
+    // ---- the rows' results ----
+    const int h = lane >> 5;
+    // m: the references in log2 units, -inf where the row has seen no key
+    float l[2] = {pair_sum(wv.l[0]), pair_sum(wv.l[1])}, m[2] = {wv.m[0] == -INFINITY ? -INFINITY : wv.mc[0], wv.m[1] == -INFINITY ? -INFINITY : wv.mc[1]};
+    constexpr int OWN = KEYS ? (NC + W - 1) / W : NC, OSTEP = KEYS ? W : 1;
+    const int own0 = KEYS ? wave : 0;
+    f32x16 o[2][OWN];
+    if constexpr (KEYS && W > 1) {
+        // every wave's share against the rows' common maxima, then block cb of all of them summed by wave cb mod W
+        float* f = (float*)lds;
+        float* stat = f + W * 2 * NC * 16 * 64;                            // [wave][map][32] maxima, then sums
+        __syncthreads();
+        if (h == 0) stat[(wave * 2 + 0) * 32 + lane] = m[0], stat[(wave * 2 + 1) * 32 + lane] = m[1];
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            float mx = -INFINITY;
+            for (int w = 0; w < W; ++w) mx = fmaxf(mx, stat[(w * 2 + y) * 32 + (lane & 31)]);
+            const float g = m[y] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[y] - mx);
+            m[y] = mx;
+            l[y] *= g;
+#pragma unroll
+            for (int cb = 0; cb < NC; ++cb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) f[(((wave * 2 + y) * NC + cb) * 16 + e) * 64 + lane] = wv.o[y][cb][e] * g;
+        }
+        __syncthreads();
+        if (h == 0) stat[(wave * 2 + 0) * 32 + lane] = l[0], stat[(wave * 2 + 1) * 32 + lane] = l[1];
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            l[y] = 0.f;
+            for (int w = 0; w < W; ++w) l[y] += stat[(w * 2 + y) * 32 + (lane & 31)];
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) {
+                const int cb = min(own0 + k * OSTEP, NC - 1);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float t = 0.f;
+                    for (int w = 0; w < W; ++w) t += f[(((w * 2 + y) * NC + cb) * 16 + e) * 64 + lane];
+                    o[y][k][e] = t;
+                }
+            }
+        }
+        __syncthreads();                                                   // stat is used once more below
+    } else {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) o[y][k] = wv.o[y][k];
+    }
+
+    if (x.splits > 1) {
+        const int64_t slot = ((int64_t)(at.b * a.kv_heads + at.hk) * x.splits + at.split) * x.rows + rr;
+        float* part = x.ws + slot * 4 * D;
+        float* stat = x.ws + part_rows(x) * 4 * D + slot * 4;
+        if (live) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int k = 0; k < OWN; ++k) {
+                    const int cb = own0 + k * OSTEP;
+                    if (cb >= NC) break;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<f32x4*>(part + y * 2 * D + cb * 32 + 8 * g + 4 * h) = f32x4{o[y][k][4 * g], o[y][k][4 * g + 1], o[y][k][4 * g + 2], o[y][k][4 * g + 3]};
+                }
+            if (h == 0 && own0 == 0) *reinterpret_cast<f32x4*>(stat) = f32x4{m[0], m[1], l[0], l[1]};
+        }
+        return;
+    }
+    float lambda = 0.f;
+    if (a.lambda_head_stride == 0) lambda = head_lambda(a, 0, lane);
+    else
+        for (int g = 0; g < x.group; ++g) {
+            const float v = head_lambda(a, at.hk * x.group + g, lane);
+            if (rr % x.group == g) lambda = v;
+        }
+    const float r0 = l[0] == 0.f ? 0.f : 1.f / l[0], r1 = l[1] == 0.f ? 0.f : lambda / l[1];
     float ss = 0.f;
-    for (int y = 0; y < 4; ++y) {
-        o[0][y] = o[0][y] * r1 - o[1][y] * r2;
-        if (lane + 64 * y < w) ss += o[0][y] * o[0][y];
+#pragma unroll
+    for (int k = 0; k < OWN; ++k)
+        if (own0 + k * OSTEP < NC) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[0][k][e] = o[0][k][e] * r0 - o[1][k][e] * r1;
+                ss = fmaf(o[0][k][e], o[0][k][e], ss);
+            }
+        }
+    ss = pair_sum(ss);
+    if constexpr (KEYS && W > 1) {
+        float* stat = (float*)lds + W * 2 * NC * 16 * 64;
+        if (h == 0) stat[wave * 32 + lane] = ss;
+        __syncthreads();
+        ss = 0.f;
+        for (int w = 0; w < W; ++w) ss += stat[w * 32 + (lane & 31)];
     }
-    float f = a.out_scale;
-    if (a.norm_weight_dev) f /= sqrtf(wave_sum(ss) / (float)w + a.norm_eps);
-    T* out = (T*)a.out_dev + b * a.out_batch_stride + i * a.out_token_stride + h * a.out_head_stride;
-    for (int y = 0; y < 4 && lane + 64 * y < w; ++y) {
-        const int col = lane + 64 * y;
-        out[col] = from_f32<T>(o[0][y] * f * (a.norm_weight_dev ? a.norm_weight_dev[col] : 1.f));
+    Out<T, D>::template store<OSTEP, OWN>(x, o[0], own0, at.b, i, head, live, norm_factor(a, ss), h);
+}
+
+// joins the splits of a query row and head: one wave, a lane owns 4 D / 128 neighbouring columns of both maps
+template <typename T, int D> __global__ __launch_bounds__(256) void diff_attention_join_kernel(const Args x) {
+    constexpr int N = 2 * D / 64;
+    const rz_diff_attention_args& a = x.a;
+    const int lane = threadIdx.x & 63;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (int64_t)a.batch * a.kv_heads * x.rows) return;
+    const int row = (int)(id % x.rows), bh = (int)(id / x.rows), b = bh / a.kv_heads, i = row / x.group, head = (bh % a.kv_heads) * x.group + row % x.group;
+    const int64_t slot = (int64_t)bh * x.splits * x.rows + row;
+    const float* part = x.ws + slot * 4 * D + lane * N;
+    const float* stat = x.ws + part_rows(x) * 4 * D + slot * 4;
+    f32x4 st = {-INFINITY, -INFINITY, 0.f, 0.f};
+    if (lane < x.splits) st = *reinterpret_cast<const f32x4*>(stat + (int64_t)lane * x.rows * 4);      // at most 64 splits
+    const float m0 = wave_max(st[0]), m1 = wave_max(st[1]);
+    const float f0 = st[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[0] - m0), f1 = st[1] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[1] - m1);
+    const float l0 = wave_sum(st[2] * f0), l1 = wave_sum(st[3] * f1);
+    float o[2][N] = {};
+    for (int s = 0; s < x.splits; ++s) {
+        const float w0 = __shfl(f0, s, 64), w1 = __shfl(f1, s, 64);
+        const float* p = part + (int64_t)s * x.rows * 4 * D;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            o[0][e] = fmaf(p[e], w0, o[0][e]);
+            o[1][e] = fmaf(p[2 * D + e], w1, o[1][e]);
+        }
     }
+    const float lambda = head_lambda(a, head, lane);
+    const float r0 = l0 == 0.f ? 0.f : 1.f / l0, r1 = l1 == 0.f ? 0.f : lambda / l1;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        o[0][e] = o[0][e] * r0 - o[1][e] * r1;
+        ss = fmaf(o[0][e], o[0][e], ss);
+    }
+    const float f = norm_factor(a, wave_sum(ss));
+    T* out = (T*)a.out_dev + b * a.out_batch_stride + i * a.out_token_stride + head * a.out_head_stride + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = from_f32<T>(o[0][e] * f * (a.norm_weight_dev ? a.norm_weight_dev[lane * N + e] : 1.f));
+}
+
+int cu_count() {
+    static const int n = [] {
+        int dev = 0, v = 0;
+        if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) v = 256;
+        return v;
+    }();
+    return n;
+}
+
+// Few rows: the waves of a workgroup share the rows and split the keys.  Keys are split over workgroups too while CUs would stand idle and a split keeps
+// 4 tiles for every wave; at most 64 splits (the join reads them by one wave).
+Plan plan(const rz_diff_attention_args& a) {
+    const int rows = a.n_q * (a.heads / a.kv_heads);
+    Plan p;
+    p.keys_mode = rows <= 32;
+    const int64_t base = (int64_t)a.batch * a.kv_heads * (p.keys_mode ? 1 : (rows + 127) / 128);
+    const int64_t want = (int64_t)2 * cu_count();
+    const int least = p.keys_mode ? 512 : 256;
+    int64_t s = base * 4 > want * 3 ? 1 : want / base;
+    s = min(s, (int64_t)a.n_k / least);
+    p.splits = (int)max((int64_t)1, min(s, (int64_t)64));
+    return p;
+}
+
+Args make(const rz_diff_attention_args& a, const Plan& p, void* ws) {
+    Args x;
+    x.a = a;
+    x.group = a.heads / a.kv_heads;
+    x.rows = a.n_q * x.group;
+    x.row_blocks = p.keys_mode ? (x.rows + 31) / 32 : (x.rows + 127) / 128;
+    x.splits = p.splits;
+    x.ws = (float*)ws;
+    return x;
+}
+
+template <typename T, int D> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
+    typedef Shape<T, D> S;
+    const Plan p = plan(a);
+    const Args x = make(a, p, ws);
+    const dim3 grid((unsigned)((int64_t)x.row_blocks * x.splits * a.kv_heads * a.batch));
+    if (p.keys_mode) {
+        constexpr int W = keys_waves<T, D>();
+        // the join of W waves: their O and 3 x 64 floats of statistics each, where W > 1
+        constexpr int tiles = W * 4 * 32 * S::RB, join = W > 1 ? W * (2 * 2 * D * 32 + 64) * 4 : 0;
+        constexpr int bytes = tiles > join ? tiles : join;
+        static_assert(bytes <= 160 * 1024, "LDS");
+        auto* k = diff_attention_kernel<T, D, true>;
+        static const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(k, grid, dim3(64 * W), bytes, s, x);
+    } else {
+        constexpr int bytes = 4 * rows_tile<T, D>() * S::RB;
+        static_assert(bytes <= 160 * 1024, "LDS");
+        auto* k = diff_attention_kernel<T, D, false>;
+        static const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(k, grid, dim3(64 * kRowsWaves), bytes, s, x);
+    }
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || x.splits == 1) return e;
+    hipLaunchKernelGGL((diff_attention_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.batch * a.kv_heads * x.rows + 3) / 4)), dim3(256), 0, s, x);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
+    return a.head_dim == 32 ? launch<T, 32>(a, ws, s) : a.head_dim == 64 ? launch<T, 64>(a, ws, s) : launch<T, 128>(a, ws, s);
 }
 
 }  // namespace
 
-size_t diff_attention_workspace_bytes(const rz_diff_attention_args&) { return 0; }
+size_t diff_attention_workspace_bytes(const rz_diff_attention_args& a) {
+    const Args x = make(a, plan(a), nullptr);
+    return x.splits > 1 ? (size_t)part_rows(x) * (4 * a.head_dim + 4) * sizeof(float) : 0;
+}
 
-hipError_t launch_diff_attention(const rz_diff_attention_args& a, void*, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)a.batch * a.n_q * a.heads));
-    if (a.dtype == DT_F32) hipLaunchKernelGGL(diff_attention_kernel<float>, grid, dim3(64), 0, s, a);
-    else if (a.dtype == DT_BF16) hipLaunchKernelGGL(diff_attention_kernel<bf16_t>, grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL(diff_attention_kernel<f16_t>, grid, dim3(64), 0, s, a);
-    return hipGetLastError();
+hipError_t launch_diff_attention(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
+    return a.dtype == DT_F32 ? launch<float>(a, ws, s) : a.dtype == DT_BF16 ? launch<bf16_t>(a, ws, s) : launch<f16_t>(a, ws, s);
 }
 
 }  // namespace rz
