@@ -55,6 +55,15 @@ __device__ __forceinline__ float pair_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// LDS by 32-bit address: a fragment's place is a lane's constant XOR a constant of the step, plus an offset the instruction carries
+template <typename V> __device__ __forceinline__ V lds_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)at; }
+__device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+// A lane number that the compiler takes to be new: what is computed from it is computed where it stands, and does not hold registers across the loop.
+__device__ __forceinline__ int fresh(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 template <typename T, int D> struct Shape {
     static constexpr int RB = 2 * D * (int)sizeof(T);          // bytes of a key's row: both maps' halves; the same for its values
     static constexpr int CH = RB / 16;                         // 16-byte chunks of a row
@@ -102,8 +111,6 @@ __device__ __forceinline__ float head_lambda(const rz_diff_attention_args& a, in
 template <typename T, int D> struct Wave {
     typedef Shape<T, D> S;
     typedef typename Op<T>::chunk chunk;
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef short s16x8 __attribute__((ext_vector_type(8)));
     static constexpr int NT = S::NT, NC = S::NC, RB = S::RB;
 
     chunk q[2][NT];
@@ -128,14 +135,15 @@ template <typename T, int D> struct Wave {
         }
     }
 
-    // S^T of 32 keys: register e is key 8 (e / 4) + 4 h + e % 4 of them
-    __device__ __forceinline__ f32x16 scores(const char* kt, int y) const {
-        f32x16 s = {};
+    // S^T of the 32 keys at kt (k_lane() of their LDS image): register e is key 8 (e / 4) + 4 h + e % 4 of them
+    static __device__ __forceinline__ uint32_t k_lane(int lane) {
         const int r = lane & 31;
-        const char* row = kt + r * RB;
-        const int x = S::swz_k(r);
+        return r * RB + (((lane >> 5) ^ S::swz_k(r)) << 4);
+    }
+    __device__ __forceinline__ f32x16 scores(uint32_t kt, int y) const {
+        f32x16 s = {};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s = Op<T>::mma(*reinterpret_cast<const chunk*>(row + (((y * NT + t) * 2 + h) ^ x) * 16), q[y][t], s);
+        for (int t = 0; t < NT; ++t) s = Op<T>::mma(lds_read<chunk>(kt ^ ((y * NT + t) << 5)), q[y][t], s);
         return s;
     }
 
@@ -172,20 +180,30 @@ template <typename T, int D> struct Wave {
         return t0 + t1;
     }
 
-    // O^T += V^T P^T for both maps
-    __device__ __forceinline__ void values(const char* vt, const f32x16 (&p)[2]) {
+    // O^T += V^T P^T for both maps, the values of 32 keys at vt (v_lane() of their LDS image)
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ s16x4 tr(uint32_t at) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at); }
+    static __device__ __forceinline__ uint32_t v_lane(int lane) {
+        const int h = lane >> 5;
         if constexpr (sizeof(T) == 4) {
             const int col = lane & 31;
+            return 4 * h * RB + (((col >> 2) ^ S::swz_v(4 * h)) << 4) + (col & 3) * 4;
+        } else {
+            // a transposing read gives lane x of 16 column x of 4 rows; the lanes of a group point at those rows, 4 lanes (32 bytes) each
+            const int x = lane & 15, sub = (lane >> 4) & 1, r0 = 4 * h + (x >> 2);
+            return r0 * RB + (((sub * 2 + ((x & 3) >> 1)) ^ S::swz_v(x >> 2)) << 4) + (x & 1) * 8;
+        }
+    }
+    __device__ __forceinline__ void values(uint32_t vt, const f32x16 (&p)[2]) {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int r = 8 * (e / 4) + 4 * h + e % 4;
+            for (int e = 0; e < 16; ++e)
 #pragma unroll
                 for (int cb = 0; cb < NC; ++cb) {
-                    const float v = *reinterpret_cast<const float*>(vt + r * RB + (((cb * 8 + (col >> 2)) ^ S::swz_v(r)) << 4) + (col & 3) * 4);
+                    const float v = lds_read<float>((vt ^ ((cb & 1) << 7)) + (cb >> 1) * 256 + (8 * (e / 4) + e % 4) * RB);
                     o[0][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[0][e], o[0][cb], 0, 0, 0);
                     o[1][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[1][e], o[1][cb], 0, 0, 0);
                 }
-            }
         } else {
             chunk w[2][2];
 #pragma unroll
@@ -193,25 +211,21 @@ template <typename T, int D> struct Wave {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     w[y][u] = pack8<T>(p[y][8 * u], p[y][8 * u + 1], p[y][8 * u + 2], p[y][8 * u + 3], p[y][8 * u + 4], p[y][8 * u + 5], p[y][8 * u + 6], p[y][8 * u + 7]);
-            // a transposing read gives lane x of 16 column x of 4 rows; the lanes of a group point at those rows, 4 lanes (32 bytes) each
-            const int x = lane & 15, sub = (lane >> 4) & 1, r0 = 4 * h + (x >> 2), swz = S::swz_v(x >> 2);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int cb = 0; cb < NC; ++cb) {
-                    const char* at = vt + r0 * RB + (((cb * 4 + sub * 2 + ((x & 3) >> 1)) ^ swz) << 4) + (x & 1) * 8;
-                    const s16x4 a = tr(at + (16 * u) * RB), b = tr(at + (16 * u + 8) * RB);
-                    const chunk v = __builtin_bit_cast(chunk, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+                    const uint32_t at = (vt ^ ((cb & 3) << 6)) + (cb >> 2) * 256 + 16 * u * RB;
+                    const chunk v = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at), tr(at + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
                     o[0][cb] = Op<T>::mma(v, w[0][u], o[0][cb]);
                     o[1][cb] = Op<T>::mma(v, w[1][u], o[1][cb]);
                 }
         }
     }
-    static __device__ __forceinline__ s16x4 tr(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p); }
 
     // 32 keys that stand in LDS at kt, vt.  seen: bit j = this lane's query sees key j; all: every query of the wave sees every key;
     // odd: bit j = key j's values were not all finite (take_odd)
-    __device__ __forceinline__ void block(const char* kt, const char* vt, uint32_t seen, bool all, uint32_t odd) {
+    __device__ __forceinline__ void block(uint32_t kt, uint32_t vt, uint32_t seen, bool all, uint32_t odd) {
         f32x16 s[2];
         float t[2];
         bool fine = false;
@@ -226,12 +240,11 @@ template <typename T, int D> struct Wave {
         if (!fine) {
             // Hardly ever taken: one map after the other, on fragments read anew.  What the path above holds is not kept for this one (registers).
             const uint32_t mine = seen >> (4 * h);
-            int zero = 0;
-            asm("" : "+v"(zero));
+            const uint32_t again = (uint32_t)fresh((int)kt);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 __builtin_amdgcn_sched_barrier(0);
-                s[y] = scores(kt + zero, y);
+                s[y] = scores(again, y);
                 recentre(s[y], y, mine);
                 t[y] = weights(s[y], y);
             }
@@ -248,6 +261,18 @@ template <typename T, int D> struct Wave {
 // bits of the keys below `n` (any n)
 __device__ __forceinline__ uint64_t below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
+// LDS-DMA of 16 bytes per lane to 1 KB at `lds` (wave-uniform), from a uniform address plus a lane's offset, or from a lane's address.  Written in assembly: the
+// compiler takes every LDS read behind its own builtin to depend on the copy and would wait for the next tile before it reads this one.  The copies have no
+// output register; whoever reads the tile waits for all of them first (landed()).  One wait state between the write of m0 and its use.
+__device__ __forceinline__ uint32_t lds_offset(char* lds) { return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds); }
+__device__ __forceinline__ void lds_dma(char* lds, const char* base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_offset(lds)), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_dma(char* lds, const char* p) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_offset(lds)), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
 // Fills LDS rows [0, ROWS) x RB bytes with keys j0 ..; wave w of W.  Keys that nobody may see (bits 0: hidden, or behind the last) are replaced by the first that
 // somebody does: their weights are 0, and 0 * (what a hidden place holds) would not be.
 template <typename T, int D, int ROWS, int W, bool VALUES>
@@ -255,14 +280,24 @@ __device__ __forceinline__ void stage(char* lds, const char* src, int64_t stride
     typedef Shape<T, D> S;
     constexpr int per = 1024 / S::RB, N = ROWS * S::RB / 1024 / W;         // rows of one LDS-DMA instruction (1 KB), instructions of a wave
     static_assert(S::RB <= 1024 && ROWS * S::RB % (1024 * W) == 0, "tile and waves do not fit");
+    lane = fresh(lane);
     const int sub = lane / S::CH, cp = lane % S::CH;
-    const int first = __builtin_ctzll(bits);
+    if (bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1)) {        // every key: a uniform address and a lane's offset that is the same in every tile
+        const uint32_t in = (uint32_t)sub * (uint32_t)stride;
+        const char* base = src + (int64_t)j0 * stride;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r0 = (w * N + i) * per, r = r0 + sub;
-        const int key = j0 + ((bits >> r) & 1 ? r : first);
-        const char* p = src + (int64_t)key * stride + ((cp ^ (VALUES ? S::swz_v(r) : S::swz_k(r))) << 4);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)(lds + r0 * S::RB), 16, 0, 0);
+        for (int i = 0; i < N; ++i) {
+            const int r0 = (w * N + i) * per, r = r0 + sub;
+            lds_dma(lds + r0 * S::RB, base + (int64_t)r0 * stride, in + ((cp ^ (VALUES ? S::swz_v(r) : S::swz_k(r))) << 4));
+        }
+    } else {
+        const int first = __builtin_ctzll(bits);
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+            const int r0 = (w * N + i) * per, r = r0 + sub;
+            const int key = j0 + ((bits >> r) & 1 ? r : first);
+            lds_dma(lds + r0 * S::RB, src + (int64_t)key * stride + ((cp ^ (VALUES ? S::swz_v(r) : S::swz_k(r))) << 4));
+        }
     }
 }
 
@@ -381,43 +416,67 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
     const int64_t* mask = a.mask_dev ? a.mask_dev + at.b * a.mask_batch_stride : nullptr;
     constexpr int STEP = KEYS ? BN * W : BN;
     const int j_first = begin + (KEYS ? wave * BN : 0);
-    // keys of the tile at j that some query may see; the mask's values are asked for one tile ahead
-    auto ask = [&](int j) -> int64_t { return mask && j + lane < stop && lane < BN ? mask[j + lane] : 0; };
-    auto answer = [&](int j, int64_t v) -> uint64_t {
-        const uint64_t in = below(min(stop - j, BN));
-        return mask ? in & __ballot(v != 0) : in;
+    // Tile k of this workgroup (wave) begins at key j_first + k STEP.  Which of its keys the mask leaves: a bit each; lane n holds those of tile chunk + n, so that
+    // a mask is read for 64 tiles at a time and an empty tile costs nothing.
+    const int tiles = (max(stop - j_first, 0) + STEP - 1) / STEP;
+    int chunk = mask ? -64 : 0;
+    uint64_t words = ~0ull;
+    auto read_mask = [&](int k) {
+        chunk = k;
+        const int here = min(tiles - k, 64);
+        words = 0;
+        constexpr int per = 64 / BN;                                       // tiles of one load
+#pragma unroll 4
+        for (int n = 0; n < here; n += per) {
+            const int key = j_first + (k + n + (per > 1 ? lane / BN : 0)) * STEP + lane % BN;
+            const uint64_t b = __ballot(key < stop && mask[key] != 0);
+            words = lane == n ? (per > 1 ? b & 0xffffffffu : b) : per > 1 && lane == n + 1 ? b >> 32 : words;
+        }
+    };
+    int k_next = 0;
+    uint64_t bits_next = 0;
+    auto find = [&] {                                                      // the first tile from k_next on that has a key
+        bits_next = 0;
+        while (k_next < tiles) {
+            if (mask) {
+                if (k_next >= chunk + 64) read_mask(k_next);
+                const uint64_t some = __ballot(words != 0) >> (k_next - chunk);
+                if (!some) {
+                    k_next = chunk + 64;
+                    continue;
+                }
+                k_next += __builtin_ctzll(some);
+                bits_next = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)words, k_next - chunk) |
+                            (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(words >> 32), k_next - chunk) << 32;
+            } else {
+                bits_next = below(min(stop - (j_first + k_next * STEP), BN));
+            }
+            return;
+        }
     };
     auto fill = [&](char* buf, int j, uint64_t bits) {
         stage<T, D, BN, KEYS ? 1 : W, false>(buf, kp, ks, j, bits, KEYS ? 0 : wave, lane);
         stage<T, D, BN, KEYS ? 1 : W, true>(buf + TILE, vp, vs, j, bits, KEYS ? 0 : wave, lane);
     };
     char* mine = lds + (KEYS ? wave * 2 * BUF : 0);
-    // the next tile with a key that somebody sees
-    int j_next = j_first;
-    uint64_t bits_next = answer(j_next, ask(j_next));
-    int64_t asked = ask(j_next + STEP);
-    auto skip_empty = [&] {
-        while (!bits_next && j_next < stop) {
-            j_next += STEP;
-            bits_next = answer(j_next, asked);
-            asked = ask(j_next + STEP);
-        }
-    };
-    skip_empty();
-    if (bits_next) fill(mine, j_next, bits_next);
+    // the queries are there before the first copy leaves: a wait for them inside the loop would be one for the copies too
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int t = 0; t < S::NT; ++t) asm volatile("" : "+v"(wv.q[y][t]));
+    find();
+    if (bits_next) fill(mine, j_first + k_next * STEP, bits_next);
     int turn = 0;
     while (bits_next) {
-        const int j = j_next;
+        const int j = j_first + k_next * STEP;
         const uint64_t bits = bits_next;
         // everything asked for so far has landed; the other buffer's readers are done
-        if constexpr (KEYS) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        else __syncthreads();
-        j_next = j + STEP;
-        bits_next = answer(j_next, asked);
-        asked = ask(j_next + STEP);
-        skip_empty();
-        if (bits_next) fill(mine + (turn ^ 1) * BUF, j_next, bits_next);
+        landed();
+        if constexpr (!KEYS) __syncthreads();
+        ++k_next;
+        find();
         char* buf = mine + turn * BUF;
+        if (bits_next) fill(mine + (turn ^ 1) * BUF, j_first + k_next * STEP, bits_next);
         const bool all = bits == below(BN) && j + BN <= wave_first;
         uint64_t odd = 0;
         if (a.causal && j + BN > group_first) {                            // the same for all waves that share the tile
@@ -429,10 +488,12 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
                 else __syncthreads();
             }
         }
+        const int again = fresh(lane);
+        const uint32_t kt = lds_address(buf) + Wave<T, D>::k_lane(again), vt = lds_address(buf) + TILE + Wave<T, D>::v_lane(again);
 #pragma unroll
         for (int kb = 0; kb < BN / 32; ++kb) {
             const uint32_t seen = (uint32_t)((bits & below(lim - j)) >> (32 * kb));
-            wv.block(buf + kb * 32 * S::RB, buf + TILE + kb * 32 * S::RB, seen, all, (uint32_t)(odd >> (32 * kb)));
+            wv.block(kt + kb * 32 * S::RB, vt + kb * 32 * S::RB, seen, all, (uint32_t)(odd >> (32 * kb)));
         }
         turn ^= 1;
     }
