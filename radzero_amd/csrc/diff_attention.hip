@@ -78,22 +78,60 @@ template <typename T, int D> struct Shape {
     }
 };
 
-constexpr int kRowsWaves = 4;
-// keys of a tile: 64 where the tile buffers of two workgroups fit the LDS, 32 for long rows
-template <typename T, int D> constexpr int rows_tile() { return Shape<T, D>::RB <= 256 ? 64 : 32; }
-// waves that split the keys of the same rows: as many private double buffers of 32 keys as 128 KB hold
-template <typename T, int D> constexpr int keys_waves() { return Shape<T, D>::RB <= 256 ? 4 : Shape<T, D>::RB == 512 ? 2 : 1; }
-
-struct Plan { int keys_mode, splits; };
-
-struct Args {
-    rz_diff_attention_args a;
-    int group, rows, row_blocks, splits;                       // heads per key head, query rows per key head, their blocks, key splits
-    float* ws;
+// How a workgroup shares the work.  MAPS: maps of a wave.  Two share a fragment of the values; head dim 128 would need 256 registers for both O, so there
+// two waves take a map each.  BN: keys of a tile, 64 where the tile buffers of two workgroups fit the LDS, 32 for long rows.
+template <typename T, int D, bool KEYS> struct Form {
+    static constexpr int RB = Shape<T, D>::RB;
+    static constexpr int MAPS = D == 128 ? 1 : 2;
+    static constexpr int W = KEYS ? (RB <= 256 ? 4 : 2) : 4;   // keys: as many private double buffers of 32 keys as 128 KB hold
+    static constexpr int BR = KEYS ? 32 : 32 * W * MAPS / 2;   // query rows
+    static constexpr int BN = KEYS ? 32 : RB <= 256 ? 64 : 32;
+    static constexpr int TILE = BN * RB, BUF = 2 * TILE;       // keys, then values
+    static constexpr int NC = Shape<T, D>::NC;
+    static constexpr int kTiles = 2 * BUF * (KEYS ? W : 1);
+    // what the waves exchange at the end: keys, every wave's O, maxima and sums; one map per wave, the second maps' O
+    static constexpr int kJoin = KEYS ? W * (2 * 2 * D * 32 + 64) * 4 : MAPS == 1 ? W / 2 * 2 * D * 32 * 4 : 0;
+    static constexpr int kLds = kTiles > kJoin ? kTiles : kJoin;
+    // workgroups that a CU holds: LDS, and 512 registers of a SIMD lane (two waves of the 16-bit forms, three of their 64-column values, one of fp32)
+    static constexpr int kWaves = sizeof(T) == 4 ? 1 : D == 32 ? 3 : 2;
+    static constexpr int kPerCu = kWaves * 4 / W < 160 * 1024 / kLds ? kWaves * 4 / W : 160 * 1024 / kLds;
+    static_assert(kLds <= 160 * 1024 && kPerCu >= 1, "LDS");
+    static_assert(!KEYS || MAPS == 2, "one map per wave: rows only");
 };
 
-// partial results of a split, floats: [batch][kv head][split][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
-__host__ __device__ inline int64_t part_rows(const Args& x) { return (int64_t)x.a.batch * x.a.kv_heads * x.splits * x.rows; }
+// Units of work: a block of query rows of a key head.  The first `full` of them run whole, the rest are split over `splits` workgroups each.
+struct Args {
+    rz_diff_attention_args a;
+    int group, rows, row_blocks;                               // heads per key head, query rows per key head, their blocks
+    int units, full, splits;
+    int part_rows;                                             // rows of a unit in the workspace
+    float* ws;
+};
+// workspace, floats: [unit - full][split][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
+__host__ __device__ inline int64_t parts(const Args& x) { return (int64_t)(x.units - x.full) * x.splits * x.part_rows; }
+
+struct Work {
+    int unit, split, rb, hk, b;
+    bool whole;
+    __device__ __forceinline__ void place(const Args& x) {
+        rb = x.row_blocks - 1 - unit % x.row_blocks;           // row blocks innermost: they read the same keys; causal: the longest first
+        const int bh = unit / x.row_blocks;
+        hk = bh % x.a.kv_heads;
+        b = bh / x.a.kv_heads;
+    }
+    __device__ __forceinline__ Work(const Args& x) {
+        const int id = blockIdx.x;
+        whole = id < x.full;
+        if (whole) unit = xcd_remap(id, x.full), split = 0;
+        else {
+            const int t = xcd_remap(id - x.full, gridDim.x - x.full);
+            unit = x.full + t / x.splits;
+            split = t % x.splits;
+            whole = x.splits == 1;
+        }
+        place(x);
+    }
+};
 
 // lambda of query head h, by the whole wave
 __device__ __forceinline__ float head_lambda(const rz_diff_attention_args& a, int h, int lane) {
@@ -108,24 +146,24 @@ __device__ __forceinline__ float head_lambda(const rz_diff_attention_args& a, in
 }
 
 // ---- one wave's 32 query rows ---------------------------------------------------------------------------------------------------
-template <typename T, int D> struct Wave {
+template <typename T, int D, int MAPS> struct Wave {
     typedef Shape<T, D> S;
     typedef typename Op<T>::chunk chunk;
     static constexpr int NT = S::NT, NC = S::NC, RB = S::RB;
 
-    chunk q[2][NT];
-    f32x16 o[2][NC];
-    float m[2], mc[2], l[2];          // reference maximum (raw score), the same times c, this lane's share of the sum
+    chunk q[MAPS][NT];
+    f32x16 o[MAPS][NC];
+    float m[MAPS], l[MAPS];                 // reference maximum of the scores in log2 units (-inf: no key yet), this lane's share of the sum
     float c;                          // scale * log2(e)
-    int lane, h;                      // h: which half of every 8 keys the lane holds
+    int h;                            // which half of every 8 keys the lane holds
     bool started;                     // every row has a reference maximum (wave-uniform)
 
-    __device__ __forceinline__ void init(const Args& x, const T* qrow) {
+    __device__ __forceinline__ void init(const Args& x, const T* qrow) {      // qrow: the first of the wave's maps
         c = x.a.scale * 1.44269504088896340736f;
         started = false;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            m[y] = -INFINITY, mc[y] = 0.f, l[y] = 0.f;
+        for (int y = 0; y < MAPS; ++y) {
+            m[y] = -INFINITY, l[y] = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) q[y][t] = *reinterpret_cast<const chunk*>((const char*)qrow + (y * NT + t) * 32 + h * 16);
 #pragma unroll
@@ -147,40 +185,60 @@ template <typename T, int D> struct Wave {
         return s;
     }
 
-    // a first tile, a tile with hidden keys, or one whose weights outgrew the reference: the maximum is taken, O and l follow it
-    __device__ __forceinline__ void recentre(f32x16& s, int y, uint32_t seen) {
+    // hides keys, and where `need` (a row's first keys, or weights that outgrew the reference) takes the maximum anew; O and l follow it
+    __device__ __forceinline__ void recentre(f32x16& s, int y, uint32_t seen, bool need) {
         float mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             s[e] = (seen >> (8 * (e / 4) + e % 4)) & 1 ? s[e] : -INFINITY;
             mx = fmaxf(mx, s[e]);
         }
-        const float mn = fmaxf(m[y], pair_max(mx));
+        const float top = pair_max(mx) * c, mn = need ? fmaxf(m[y], top) : m[y];
         if (__any(mn > m[y])) {
-            const float mcn = mn == -INFINITY ? 0.f : mn * c, f = m[y] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc[y] - mcn);      // m == mn: 1
+            const float f = m[y] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[y] - mn);            // m == mn: 1
             l[y] *= f;
 #pragma unroll
             for (int cb = 0; cb < NC; ++cb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[y][cb][e] *= f;
             m[y] = mn;
-            mc[y] = mcn;
         }
     }
 
-    __device__ __forceinline__ float weights(f32x16& s, int y) const {
-        float t0 = 0.f, t1 = 0.f;
+    __device__ __forceinline__ void exponentials(f32x16& s, float reference) const {
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -mc[y]));
-            s[e + 1] = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c, -mc[y]));
-            t0 += s[e];
-            t1 += s[e + 1];
-        }
-        return t0 + t1;
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -reference));
+    }
+    // a hidden key's weight to +0, whatever it is
+    static __device__ __forceinline__ void hide(f32x16& p, uint32_t seen) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = __uint_as_float(__float_as_uint(p[e]) & (uint32_t)__builtin_amdgcn_sbfe((int)seen, 8 * (e / 4) + e % 4, 1));
+    }
+    static __device__ __forceinline__ float sum(const f32x16& p) {
+        float t[2] = {p[0], p[1]};
+#pragma unroll
+        for (int e = 2; e < 16; ++e) t[e & 1] += p[e];
+        return t[0] + t[1];
     }
 
-    // O^T += V^T P^T for both maps, the values of 32 keys at vt (v_lane() of their LDS image)
+    // The weights of 32 keys without a maximum: one that outgrows the reference shows in the sum.  2^15 keeps every weight below the largest f16.  False: some row's did.
+    // One run of instructions from the matrix products to what reads them: with a branch between, the fp32 kernels came out without the wait states they need.
+    static constexpr float kMost = 32768.f;
+    template <bool HIDE> __device__ __forceinline__ bool straight(uint32_t kt, uint32_t seen, f32x16 (&s)[MAPS], float (&t)[MAPS], bool& fine) const {
+#pragma unroll
+        for (int y = 0; y < MAPS; ++y) s[y] = scores(kt, y);
+        fine = true;
+#pragma unroll
+        for (int y = 0; y < MAPS; ++y) {
+            exponentials(s[y], m[y]);
+            if constexpr (HIDE) hide(s[y], seen);
+            t[y] = sum(s[y]);
+            fine = fine && t[y] <= kMost;
+        }
+        return !__any(!fine);
+    }
+
+    // O^T += V^T P^T, the values of 32 keys at vt (v_lane() of their LDS image)
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ s16x4 tr(uint32_t at) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at); }
     static __device__ __forceinline__ uint32_t v_lane(int lane) {
@@ -194,20 +252,20 @@ template <typename T, int D> struct Wave {
             return r0 * RB + (((sub * 2 + ((x & 3) >> 1)) ^ S::swz_v(x >> 2)) << 4) + (x & 1) * 8;
         }
     }
-    __device__ __forceinline__ void values(uint32_t vt, const f32x16 (&p)[2]) {
+    __device__ __forceinline__ void values(uint32_t vt, const f32x16 (&p)[MAPS]) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
 #pragma unroll
                 for (int cb = 0; cb < NC; ++cb) {
                     const float v = lds_read<float>((vt ^ ((cb & 1) << 7)) + (cb >> 1) * 256 + (8 * (e / 4) + e % 4) * RB);
-                    o[0][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[0][e], o[0][cb], 0, 0, 0);
-                    o[1][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[1][e], o[1][cb], 0, 0, 0);
+#pragma unroll
+                    for (int y = 0; y < MAPS; ++y) o[y][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[y][e], o[y][cb], 0, 0, 0);
                 }
         } else {
-            chunk w[2][2];
+            chunk w[MAPS][2];
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+            for (int y = 0; y < MAPS; ++y)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     w[y][u] = pack8<T>(p[y][8 * u], p[y][8 * u + 1], p[y][8 * u + 2], p[y][8 * u + 3], p[y][8 * u + 4], p[y][8 * u + 5], p[y][8 * u + 6], p[y][8 * u + 7]);
@@ -217,8 +275,8 @@ template <typename T, int D> struct Wave {
                 for (int cb = 0; cb < NC; ++cb) {
                     const uint32_t at = (vt ^ ((cb & 3) << 6)) + (cb >> 2) * 256 + 16 * u * RB;
                     const chunk v = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at), tr(at + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
-                    o[0][cb] = Op<T>::mma(v, w[0][u], o[0][cb]);
-                    o[1][cb] = Op<T>::mma(v, w[1][u], o[1][cb]);
+#pragma unroll
+                    for (int y = 0; y < MAPS; ++y) o[y][cb] = Op<T>::mma(v, w[y][u], o[y][cb]);
                 }
         }
     }
@@ -226,34 +284,41 @@ template <typename T, int D> struct Wave {
     // 32 keys that stand in LDS at kt, vt.  seen: bit j = this lane's query sees key j; all: every query of the wave sees every key;
     // odd: bit j = key j's values were not all finite (take_odd)
     __device__ __forceinline__ void block(uint32_t kt, uint32_t vt, uint32_t seen, bool all, uint32_t odd) {
-        f32x16 s[2];
-        float t[2];
-        bool fine = false;
-        if (all && started) {
-            // No maximum here: a weight that outgrows the reference shows in the sum.  2^15 keeps every weight below the largest f16.
-            s[0] = scores(kt, 0);
-            s[1] = scores(kt, 1);
-            t[0] = weights(s[0], 0);
-            t[1] = weights(s[1], 1);
-            fine = !__any(!(t[0] <= 32768.f && t[1] <= 32768.f));
-        }
-        if (!fine) {
-            // Hardly ever taken: one map after the other, on fragments read anew.  What the path above holds is not kept for this one (registers).
-            const uint32_t mine = seen >> (4 * h);
-            const uint32_t again = (uint32_t)fresh((int)kt);
+        f32x16 s[MAPS];
+        float t[MAPS];
+        const uint32_t mine = seen >> (4 * h);
+        bool done = false, fine = true;
+        if (started) done = all ? straight<false>(kt, mine, s, t, fine) : straight<true>(kt, mine, s, t, fine);
+        if (!done) {
+            // Hardly ever taken: one map after the other, on fragments read anew.  What the path above holds is not kept for this one (registers).  A row is centred
+            // anew for its own sake alone: its result does not depend on the rows beside it.
+            bool need = !fine;
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
+            for (int y = 0; y < MAPS; ++y) need = need || m[y] == -INFINITY;
+            for (bool more = true; more;) {
+                need = pair_max(need ? 1.f : 0.f) > 0.f;
+                const uint32_t again = (uint32_t)fresh((int)kt);
+                started = true;
+                bool over = false;
+#pragma unroll
+                for (int y = 0; y < MAPS; ++y) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    s[y] = scores(again, y);
+                    recentre(s[y], y, mine, need);
+                    exponentials(s[y], m[y] == -INFINITY ? 0.f : m[y]);
+                    t[y] = sum(s[y]);
+                    over = over || !(t[y] <= kMost);
+                    started = started && __all(m[y] > -INFINITY);
+                }
                 __builtin_amdgcn_sched_barrier(0);
-                s[y] = scores(again, y);
-                recentre(s[y], y, mine);
-                t[y] = weights(s[y], y);
+                over = over && !need;                                      // seen while another row's first keys were: once more, for it
+                more = __any(over);
+                need = need || over;
             }
-            __builtin_amdgcn_sched_barrier(0);
-            started = __all(m[0] > -INFINITY && m[1] > -INFINITY);
         }
         const float poison = seen & odd ? __builtin_nanf("") : 0.f;
-        l[0] += t[0] + poison;
-        l[1] += t[1];
+#pragma unroll
+        for (int y = 0; y < MAPS; ++y) l[y] += t[y] + poison;
         values(vt, s);
     }
 };
@@ -362,53 +427,40 @@ __device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, fl
     return a.norm_weight_dev ? a.out_scale / sqrtf(sum_of_squares / (float)(2 * a.head_dim) + a.norm_eps) : a.out_scale;
 }
 
-// What a workgroup works on, from its id: row blocks innermost (they read the same keys), then splits, then key heads
-struct Work {
-    int rb, split, hk, b;
-    __device__ __forceinline__ Work(const Args& x) {
-        int id = xcd_remap(blockIdx.x, gridDim.x);
-        rb = x.row_blocks - 1 - id % x.row_blocks;                         // causal: the longest first
-        id /= x.row_blocks;
-        split = id % x.splits;
-        id /= x.splits;
-        hk = id % x.a.kv_heads;
-        b = id / x.a.kv_heads;
-    }
-};
-
-template <typename T, int D, bool KEYS, int MINW = (sizeof(T) == 2 && D <= 64 ? 2 : 1)>
-__global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW) void diff_attention_kernel(const Args x) {
+template <typename T, int D, bool KEYS, typename F = Form<T, D, KEYS>>
+__global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attention_kernel(const Args x) {
     typedef Shape<T, D> S;
-    constexpr int W = KEYS ? keys_waves<T, D>() : kRowsWaves, BN = KEYS ? 32 : rows_tile<T, D>(), TILE = BN * S::RB, NC = S::NC;
-    constexpr int BUF = 2 * TILE;                                          // keys, then values
+    constexpr int W = F::W, BN = F::BN, TILE = F::TILE, BUF = F::BUF, NC = F::NC, MAPS = F::MAPS;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const rz_diff_attention_args& a = x.a;
     const Work at(x);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row0 = at.rb * (KEYS ? 32 : 32 * W) + (KEYS ? 0 : 32 * wave), row = row0 + (lane & 31);
-    const bool live = row < x.rows;
-    const int rr = min(row, x.rows - 1), i = rr / x.group, head = at.hk * x.group + rr % x.group;
+    const int map = MAPS == 1 ? wave & 1 : 0, group = KEYS ? 0 : MAPS == 1 ? wave >> 1 : wave;      // the wave's (first) map, its 32 rows of the unit
+    const int row0 = at.rb * F::BR + 32 * group;
 
     int n = a.n_k;
     if (a.kv_lens_dev) n = min(max(a.kv_lens_dev[at.b], 0), n);
     const int shift = a.causal == RZ_CAUSAL_END ? n - a.n_q : 0;
     auto limit = [&](int query) { return a.causal ? min(n, query + 1 + shift) : n; };       // keys that a query may see at most (may be negative)
-    const int lim = limit(i);
-    const int last = min(at.rb * (KEYS ? 32 : 32 * W) + (KEYS ? 32 : 32 * W), x.rows) - 1;
+    int lim;
+    const int last = min((at.rb + 1) * F::BR, x.rows) - 1;
     const int end = max(limit(last / x.group), 0);                         // of the workgroup
     const int wave_first = limit(min(row0, x.rows - 1) / x.group);         // keys that every query of the wave sees, but for hidden ones
-    const int group_first = limit(at.rb * (KEYS ? 32 : 32 * W) / x.group); // the same of the workgroup
+    const int unit_first = limit(at.rb * F::BR / x.group);                 // the same of the workgroup
     int begin = 0, stop = end;
-    if (x.splits > 1) {
+    if (!at.whole) {
         const int per = ((end + x.splits - 1) / x.splits + 63) / 64 * 64;
         begin = min(at.split * per, end);
         stop = min(begin + per, end);
     }
 
-    Wave<T, D> wv;
-    wv.lane = lane;
+    Wave<T, D, MAPS> wv;
     wv.h = lane >> 5;
-    wv.init(x, (const T*)a.q_dev + at.b * a.q_batch_stride + i * a.q_token_stride + head * a.q_head_stride);
+    {
+        const int rr = min(row0 + (lane & 31), x.rows - 1), i = rr / x.group, head = at.hk * x.group + rr % x.group;
+        lim = limit(i);
+        wv.init(x, (const T*)a.q_dev + at.b * a.q_batch_stride + i * a.q_token_stride + head * a.q_head_stride + map * D);
+    }
 
     const char* kp = (const char*)((const T*)a.k_dev + at.b * a.k_batch_stride + at.hk * a.k_head_stride);
     const char* vp = (const char*)((const T*)a.v_dev + at.b * a.v_batch_stride + at.hk * a.v_head_stride);
@@ -461,7 +513,7 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
     char* mine = lds + (KEYS ? wave * 2 * BUF : 0);
     // the queries are there before the first copy leaves: a wait for them inside the loop would be one for the copies too
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < MAPS; ++y)
 #pragma unroll
         for (int t = 0; t < S::NT; ++t) asm volatile("" : "+v"(wv.q[y][t]));
     find();
@@ -479,7 +531,7 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
         if (bits_next) fill(mine + (turn ^ 1) * BUF, j_first + k_next * STEP, bits_next);
         const bool all = bits == below(BN) && j + BN <= wave_first;
         uint64_t odd = 0;
-        if (a.causal && j + BN > group_first) {                            // the same for all waves that share the tile
+        if (a.causal && j + BN > unit_first) {                            // the same for all waves that share the tile
             odd = odd_keys<T, D, BN>(buf + TILE, lane);
             if (odd) {
                 if constexpr (!KEYS) __syncthreads();
@@ -489,7 +541,7 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
             }
         }
         const int again = fresh(lane);
-        const uint32_t kt = lds_address(buf) + Wave<T, D>::k_lane(again), vt = lds_address(buf) + TILE + Wave<T, D>::v_lane(again);
+        const uint32_t kt = lds_address(buf) + Wave<T, D, MAPS>::k_lane(again) + map * (S::RB / 2), vt = lds_address(buf) + TILE + Wave<T, D, MAPS>::v_lane(again);
 #pragma unroll
         for (int kb = 0; kb < BN / 32; ++kb) {
             const uint32_t seen = (uint32_t)((bits & below(lim - j)) >> (32 * kb));
@@ -499,15 +551,18 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
     }
 
     // ---- the rows' results ----
-    const int h = lane >> 5;
-    // m: the references in log2 units, -inf where the row has seen no key
-    float l[2] = {pair_sum(wv.l[0]), pair_sum(wv.l[1])}, m[2] = {wv.m[0] == -INFINITY ? -INFINITY : wv.mc[0], wv.m[1] == -INFINITY ? -INFINITY : wv.mc[1]};
+    const int again = fresh(lane), h = again >> 5, row = row0 + (again & 31), rr = min(row, x.rows - 1), i = rr / x.group, head = at.hk * x.group + rr % x.group;
+    const bool live = row < x.rows;
+    float l[MAPS], m[MAPS];
+#pragma unroll
+    for (int y = 0; y < MAPS; ++y) l[y] = pair_sum(wv.l[y]), m[y] = wv.m[y];
+    // keys: block cb of O belongs to wave cb mod W from here on, summed over all waves
     constexpr int OWN = KEYS ? (NC + W - 1) / W : NC, OSTEP = KEYS ? W : 1;
     const int own0 = KEYS ? wave : 0;
-    f32x16 o[2][OWN];
-    if constexpr (KEYS && W > 1) {
-        // every wave's share against the rows' common maxima, then block cb of all of them summed by wave cb mod W
-        float* f = (float*)lds;
+    f32x16 o[MAPS][OWN];
+    float* f = (float*)lds;
+    if constexpr (KEYS) {
+        // every wave's share against the rows' common maxima
         float* stat = f + W * 2 * NC * 16 * 64;                            // [wave][map][32] maxima, then sums
         __syncthreads();
         if (h == 0) stat[(wave * 2 + 0) * 32 + lane] = m[0], stat[(wave * 2 + 1) * 32 + lane] = m[1];
@@ -545,27 +600,30 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
         __syncthreads();                                                   // stat is used once more below
     } else {
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < MAPS; ++y)
 #pragma unroll
             for (int k = 0; k < OWN; ++k) o[y][k] = wv.o[y][k];
     }
 
-    if (x.splits > 1) {
-        const int64_t slot = ((int64_t)(at.b * a.kv_heads + at.hk) * x.splits + at.split) * x.rows + rr;
+    if (!at.whole) {
+        const int64_t slot = ((int64_t)(at.unit - x.full) * x.splits + at.split) * x.part_rows + (row - at.rb * F::BR);
         float* part = x.ws + slot * 4 * D;
-        float* stat = x.ws + part_rows(x) * 4 * D + slot * 4;
+        float* stat = x.ws + parts(x) * 4 * D + slot * 4;
         if (live) {
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+            for (int y = 0; y < MAPS; ++y)
 #pragma unroll
                 for (int k = 0; k < OWN; ++k) {
                     const int cb = own0 + k * OSTEP;
                     if (cb >= NC) break;
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
-                        *reinterpret_cast<f32x4*>(part + y * 2 * D + cb * 32 + 8 * g + 4 * h) = f32x4{o[y][k][4 * g], o[y][k][4 * g + 1], o[y][k][4 * g + 2], o[y][k][4 * g + 3]};
+                        *reinterpret_cast<f32x4*>(part + (map + y) * 2 * D + cb * 32 + 8 * g + 4 * h) = f32x4{o[y][k][4 * g], o[y][k][4 * g + 1], o[y][k][4 * g + 2], o[y][k][4 * g + 3]};
                 }
-            if (h == 0 && own0 == 0) *reinterpret_cast<f32x4*>(stat) = f32x4{m[0], m[1], l[0], l[1]};
+            if (h == 0 && own0 == 0) {
+#pragma unroll
+                for (int y = 0; y < MAPS; ++y) stat[map + y] = m[y], stat[2 + map + y] = l[y];
+            }
         }
         return;
     }
@@ -576,20 +634,42 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
             const float v = head_lambda(a, at.hk * x.group + g, lane);
             if (rr % x.group == g) lambda = v;
         }
-    const float r0 = l[0] == 0.f ? 0.f : 1.f / l[0], r1 = l[1] == 0.f ? 0.f : lambda / l[1];
-    float ss = 0.f;
+    float r[MAPS];
 #pragma unroll
-    for (int k = 0; k < OWN; ++k)
-        if (own0 + k * OSTEP < NC) {
+    for (int y = 0; y < MAPS; ++y) r[y] = l[y] == 0.f ? 0.f : (map + y ? lambda : 1.f) / l[y];
+    float ss = 0.f;
+    if constexpr (MAPS == 1) {
+        // the second map's O joins the first's in LDS
+        __syncthreads();
+        if (map) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) f[((group * NC + k) * 16 + e) * 64 + lane] = o[0][k][e] * r[0];
+        }
+        __syncthreads();
+        if (map) return;
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                o[0][k][e] = o[0][k][e] * r0 - o[1][k][e] * r1;
+                o[0][k][e] = o[0][k][e] * r[0] - f[((group * NC + k) * 16 + e) * 64 + lane];
                 ss = fmaf(o[0][k][e], o[0][k][e], ss);
             }
-        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < OWN; ++k)
+            if (own0 + k * OSTEP < NC) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    o[0][k][e] = o[0][k][e] * r[0] - o[1][k][e] * r[1];
+                    ss = fmaf(o[0][k][e], o[0][k][e], ss);
+                }
+            }
+    }
     ss = pair_sum(ss);
-    if constexpr (KEYS && W > 1) {
-        float* stat = (float*)lds + W * 2 * NC * 16 * 64;
+    if constexpr (KEYS) {
+        float* stat = f + W * 2 * NC * 16 * 64;
         if (h == 0) stat[wave * 32 + lane] = ss;
         __syncthreads();
         ss = 0.f;
@@ -599,25 +679,29 @@ __global__ __launch_bounds__(64 * (KEYS ? keys_waves<T, D>() : kRowsWaves), MINW
 }
 
 // joins the splits of a query row and head: one wave, a lane owns 4 D / 128 neighbouring columns of both maps
-template <typename T, int D> __global__ __launch_bounds__(256) void diff_attention_join_kernel(const Args x) {
+template <typename T, int D> __global__ __launch_bounds__(256) void diff_attention_join_kernel(const Args x, int block_rows) {
     constexpr int N = 2 * D / 64;
     const rz_diff_attention_args& a = x.a;
     const int lane = threadIdx.x & 63;
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (int64_t)a.batch * a.kv_heads * x.rows) return;
-    const int row = (int)(id % x.rows), bh = (int)(id / x.rows), b = bh / a.kv_heads, i = row / x.group, head = (bh % a.kv_heads) * x.group + row % x.group;
-    const int64_t slot = (int64_t)bh * x.splits * x.rows + row;
+    const int64_t tail = id / x.part_rows;
+    if (tail >= x.units - x.full) return;
+    const int unit = x.full + (int)tail, r = (int)(id - tail * x.part_rows), bh = unit / x.row_blocks;
+    const int row = (x.row_blocks - 1 - unit % x.row_blocks) * block_rows + r;
+    if (row >= x.rows) return;
+    const int b = bh / a.kv_heads, i = row / x.group, head = (bh % a.kv_heads) * x.group + row % x.group;
+    const int64_t slot = tail * x.splits * x.part_rows + r;
     const float* part = x.ws + slot * 4 * D + lane * N;
-    const float* stat = x.ws + part_rows(x) * 4 * D + slot * 4;
+    const float* stat = x.ws + parts(x) * 4 * D + slot * 4;
     f32x4 st = {-INFINITY, -INFINITY, 0.f, 0.f};
-    if (lane < x.splits) st = *reinterpret_cast<const f32x4*>(stat + (int64_t)lane * x.rows * 4);      // at most 64 splits
+    if (lane < x.splits) st = *reinterpret_cast<const f32x4*>(stat + (int64_t)lane * x.part_rows * 4);      // at most 64 splits
     const float m0 = wave_max(st[0]), m1 = wave_max(st[1]);
     const float f0 = st[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[0] - m0), f1 = st[1] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[1] - m1);
     const float l0 = wave_sum(st[2] * f0), l1 = wave_sum(st[3] * f1);
     float o[2][N] = {};
     for (int s = 0; s < x.splits; ++s) {
         const float w0 = __shfl(f0, s, 64), w1 = __shfl(f1, s, 64);
-        const float* p = part + (int64_t)s * x.rows * 4 * D;
+        const float* p = part + (int64_t)s * x.part_rows * 4 * D;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             o[0][e] = fmaf(p[e], w0, o[0][e]);
@@ -647,60 +731,58 @@ int cu_count() {
     return n;
 }
 
-// Few rows: the waves of a workgroup share the rows and split the keys.  Keys are split over workgroups too while CUs would stand idle and a split keeps
-// 4 tiles for every wave; at most 64 splits (the join reads them by one wave).
-Plan plan(const rz_diff_attention_args& a) {
-    const int rows = a.n_q * (a.heads / a.kv_heads);
-    Plan p;
-    p.keys_mode = rows <= 32;
-    const int64_t base = (int64_t)a.batch * a.kv_heads * (p.keys_mode ? 1 : (rows + 127) / 128);
-    const int64_t want = (int64_t)2 * cu_count();
-    const int least = p.keys_mode ? 512 : 256;
-    int64_t s = base * 4 > want * 3 ? 1 : want / base;
-    s = min(s, (int64_t)a.n_k / least);
-    p.splits = (int)max((int64_t)1, min(s, (int64_t)64));
-    return p;
-}
+// Few rows: the waves of a workgroup share the rows and split the keys (head dims 32 and 64).
+template <int D> bool keys_form(int rows) { return D <= 64 && rows <= 32; }
 
-Args make(const rz_diff_attention_args& a, const Plan& p, void* ws) {
+// The units fill the chip's places round by round; what is left for a last round that would leave most of it idle is split over the keys, so that its
+// splits fill one round: at most 64 of them (the join reads them by one wave), each with at least 4 tiles for every wave.
+template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& a, void* ws) {
+    typedef Form<T, D, KEYS> F;
     Args x;
     x.a = a;
     x.group = a.heads / a.kv_heads;
     x.rows = a.n_q * x.group;
-    x.row_blocks = p.keys_mode ? (x.rows + 31) / 32 : (x.rows + 127) / 128;
-    x.splits = p.splits;
+    x.row_blocks = (x.rows + F::BR - 1) / F::BR;
+    x.units = x.row_blocks * a.kv_heads * a.batch;
+    const int places = F::kPerCu * cu_count();
+    x.full = x.units / places * places;
+    const int tail = x.units - x.full;
+    x.splits = 1;
+    if (tail && (int64_t)tail * 4 <= (int64_t)places * 3) x.splits = max(1, min(min(places / tail, a.n_k / (KEYS ? 4 * F::W * F::BN : 4 * F::BN)), 64));
+    if (x.splits == 1) x.full = x.units;
+    x.part_rows = min(x.rows, F::BR);
     x.ws = (float*)ws;
     return x;
 }
 
-template <typename T, int D> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
-    typedef Shape<T, D> S;
-    const Plan p = plan(a);
-    const Args x = make(a, p, ws);
-    const dim3 grid((unsigned)((int64_t)x.row_blocks * x.splits * a.kv_heads * a.batch));
-    if (p.keys_mode) {
-        constexpr int W = keys_waves<T, D>();
-        // the join of W waves: their O and 3 x 64 floats of statistics each, where W > 1
-        constexpr int tiles = W * 4 * 32 * S::RB, join = W > 1 ? W * (2 * 2 * D * 32 + 64) * 4 : 0;
-        constexpr int bytes = tiles > join ? tiles : join;
-        static_assert(bytes <= 160 * 1024, "LDS");
-        auto* k = diff_attention_kernel<T, D, true>;
-        static const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(k, grid, dim3(64 * W), bytes, s, x);
-    } else {
-        constexpr int bytes = 4 * rows_tile<T, D>() * S::RB;
-        static_assert(bytes <= 160 * 1024, "LDS");
-        auto* k = diff_attention_kernel<T, D, false>;
-        static const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(k, grid, dim3(64 * kRowsWaves), bytes, s, x);
-    }
-    if (hipError_t e = hipGetLastError(); e != hipSuccess || x.splits == 1) return e;
-    hipLaunchKernelGGL((diff_attention_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.batch * a.kv_heads * x.rows + 3) / 4)), dim3(256), 0, s, x);
+template <typename T, int D, bool KEYS> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
+    typedef Form<T, D, KEYS> F;
+    const Args x = make<T, D, KEYS>(a, ws);
+    auto* k = diff_attention_kernel<T, D, KEYS>;
+    static const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, F::kLds);
+    if (e != hipSuccess) return e;
+    const int tail = x.units - x.full;
+    hipLaunchKernelGGL(k, dim3((unsigned)(x.full + tail * x.splits)), dim3(64 * F::W), F::kLds, s, x);
+    if (hipError_t err = hipGetLastError(); err != hipSuccess || !tail) return err;
+    hipLaunchKernelGGL((diff_attention_join_kernel<T, D>), dim3((unsigned)(((int64_t)tail * x.part_rows + 3) / 4)), dim3(256), 0, s, x, F::BR);
     return hipGetLastError();
 }
 
+template <typename T, int D> size_t workspace(const rz_diff_attention_args& a) {
+    const int rows = a.n_q * (a.heads / a.kv_heads);
+    Args x;
+    if constexpr (D <= 64) x = keys_form<D>(rows) ? make<T, D, true>(a, nullptr) : make<T, D, false>(a, nullptr);
+    else x = make<T, D, false>(a, nullptr);
+    return (size_t)parts(x) * (4 * D + 4) * sizeof(float);
+}
+template <typename T, int D> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
+    if constexpr (D <= 64)
+        if (keys_form<D>(a.n_q * (a.heads / a.kv_heads))) return launch<T, D, true>(a, ws, s);
+    return launch<T, D, false>(a, ws, s);
+}
+template <typename T> size_t workspace(const rz_diff_attention_args& a) {
+    return a.head_dim == 32 ? workspace<T, 32>(a) : a.head_dim == 64 ? workspace<T, 64>(a) : workspace<T, 128>(a);
+}
 template <typename T> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
     return a.head_dim == 32 ? launch<T, 32>(a, ws, s) : a.head_dim == 64 ? launch<T, 64>(a, ws, s) : launch<T, 128>(a, ws, s);
 }
@@ -708,8 +790,7 @@ template <typename T> hipError_t launch(const rz_diff_attention_args& a, void* w
 }  // namespace
 
 size_t diff_attention_workspace_bytes(const rz_diff_attention_args& a) {
-    const Args x = make(a, plan(a), nullptr);
-    return x.splits > 1 ? (size_t)part_rows(x) * (4 * a.head_dim + 4) * sizeof(float) : 0;
+    return a.dtype == DT_F32 ? workspace<float>(a) : a.dtype == DT_BF16 ? workspace<bf16_t>(a) : workspace<f16_t>(a);
 }
 
 hipError_t launch_diff_attention(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
