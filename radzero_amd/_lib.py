@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -171,9 +172,11 @@ class RzConfig(ctypes.Structure):
 
 
 def _struct(name, doc, *fields):
-    """A ctypes mirror of a C struct: "type name name ..." per line, types as in include/radzero_hip.h (i int32, f float, l int64, p pointer)."""
+    """A ctypes mirror of a C struct: "type name name ..." per line, types as in include/radzero_hip.h (i int32, f float, l int64, p pointer).
+    `pack` makes the same bytes from the values in order (null pointers 0): a quarter of the time, for calls whose kernels are shorter than their host side."""
     t = {"i": ctypes.c_int32, "f": ctypes.c_float, "l": ctypes.c_int64, "p": ctypes.c_void_p}
-    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": [(n, t[f.split()[0]]) for f in fields for n in f.split()[1:]]})
+    pack = struct.Struct("@" + "".join(f.split()[0].replace("l", "q").replace("p", "P") * (len(f.split()) - 1) for f in fields)).pack
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": [(n, t[f.split()[0]]) for f in fields for n in f.split()[1:]], "pack": staticmethod(pack)})
 
 
 RzRotaryArgs = _struct(

@@ -45,6 +45,37 @@ template <> struct Op<float> {
     }
 };
 
+// 32 keys' weights as the product with the values takes them, and this lane's share of their sum
+template <typename T> struct Weights {
+    typename Op<T>::chunk w[2];
+    __device__ __forceinline__ float set(const f32x16& p) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) w[u] = pack8<T>(p[8 * u], p[8 * u + 1], p[8 * u + 2], p[8 * u + 3], p[8 * u + 4], p[8 * u + 5], p[8 * u + 6], p[8 * u + 7]);
+        // the sum of the rounded weights (they then add up to one), two of them to an instruction
+        float t[2] = {0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                if constexpr (std::is_same<T, bf16_t>::value)
+                    t[u] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{w[u][e], w[u][e + 1]}, bf16x2{(bf16_t)1.f, (bf16_t)1.f}, t[u], false);
+                else
+                    t[u] = __builtin_amdgcn_fdot2(f16x2{w[u][e], w[u][e + 1]}, f16x2{(f16_t)1.f, (f16_t)1.f}, t[u], false);
+            }
+        return t[0] + t[1];
+    }
+};
+template <> struct Weights<float> {
+    f32x16 w;
+    __device__ __forceinline__ float set(const f32x16& p) {
+        w = p;
+        float t[2] = {p[0], p[1]};
+#pragma unroll
+        for (int e = 2; e < 16; ++e) t[e & 1] += p[e];
+        return t[0] + t[1];
+    }
+};
+
 // the larger of a lane and the lane 32 away, the sum of the two (both hold the same query)
 __device__ __forceinline__ float pair_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -145,6 +176,9 @@ __device__ __forceinline__ float head_lambda(const rz_diff_attention_args& a, in
     return expf(wave_sum(x1)) - expf(wave_sum(x2)) + a.lambda_init;
 }
 
+// bits of the keys below `n` (any n)
+__device__ __forceinline__ uint64_t below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+
 // ---- one wave's 32 query rows ---------------------------------------------------------------------------------------------------
 template <typename T, int D, int MAPS> struct Wave {
     typedef Shape<T, D> S;
@@ -214,17 +248,11 @@ template <typename T, int D, int MAPS> struct Wave {
 #pragma unroll
         for (int e = 0; e < 16; ++e) p[e] = __uint_as_float(__float_as_uint(p[e]) & (uint32_t)__builtin_amdgcn_sbfe((int)seen, 8 * (e / 4) + e % 4, 1));
     }
-    static __device__ __forceinline__ float sum(const f32x16& p) {
-        float t[2] = {p[0], p[1]};
-#pragma unroll
-        for (int e = 2; e < 16; ++e) t[e & 1] += p[e];
-        return t[0] + t[1];
-    }
-
     // The weights of 32 keys without a maximum: one that outgrows the reference shows in the sum.  2^15 keeps every weight below the largest f16.  False: some row's did.
     // One run of instructions from the matrix products to what reads them: with a branch between, the fp32 kernels came out without the wait states they need.
     static constexpr float kMost = 32768.f;
-    template <bool HIDE> __device__ __forceinline__ bool straight(uint32_t kt, uint32_t seen, f32x16 (&s)[MAPS], float (&t)[MAPS], bool& fine) const {
+    template <bool HIDE> __device__ __forceinline__ bool straight(uint32_t kt, uint32_t seen, Weights<T> (&p)[MAPS], float (&t)[MAPS], bool& fine) const {
+        f32x16 s[MAPS];
 #pragma unroll
         for (int y = 0; y < MAPS; ++y) s[y] = scores(kt, y);
         fine = true;
@@ -232,7 +260,7 @@ template <typename T, int D, int MAPS> struct Wave {
         for (int y = 0; y < MAPS; ++y) {
             exponentials(s[y], m[y]);
             if constexpr (HIDE) hide(s[y], seen);
-            t[y] = sum(s[y]);
+            t[y] = p[y].set(s[y]);
             fine = fine && t[y] <= kMost;
         }
         return !__any(!fine);
@@ -252,7 +280,7 @@ template <typename T, int D, int MAPS> struct Wave {
             return r0 * RB + (((sub * 2 + ((x & 3) >> 1)) ^ S::swz_v(x >> 2)) << 4) + (x & 1) * 8;
         }
     }
-    __device__ __forceinline__ void values(uint32_t vt, const f32x16 (&p)[MAPS]) {
+    __device__ __forceinline__ void values(uint32_t vt, const Weights<T> (&p)[MAPS]) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -260,15 +288,9 @@ template <typename T, int D, int MAPS> struct Wave {
                 for (int cb = 0; cb < NC; ++cb) {
                     const float v = lds_read<float>((vt ^ ((cb & 1) << 7)) + (cb >> 1) * 256 + (8 * (e / 4) + e % 4) * RB);
 #pragma unroll
-                    for (int y = 0; y < MAPS; ++y) o[y][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[y][e], o[y][cb], 0, 0, 0);
+                    for (int y = 0; y < MAPS; ++y) o[y][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[y].w[e], o[y][cb], 0, 0, 0);
                 }
         } else {
-            chunk w[MAPS][2];
-#pragma unroll
-            for (int y = 0; y < MAPS; ++y)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    w[y][u] = pack8<T>(p[y][8 * u], p[y][8 * u + 1], p[y][8 * u + 2], p[y][8 * u + 3], p[y][8 * u + 4], p[y][8 * u + 5], p[y][8 * u + 6], p[y][8 * u + 7]);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -276,19 +298,19 @@ template <typename T, int D, int MAPS> struct Wave {
                     const uint32_t at = (vt ^ ((cb & 3) << 6)) + (cb >> 2) * 256 + 16 * u * RB;
                     const chunk v = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at), tr(at + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int y = 0; y < MAPS; ++y) o[y][cb] = Op<T>::mma(v, w[y][u], o[y][cb]);
+                    for (int y = 0; y < MAPS; ++y) o[y][cb] = Op<T>::mma(v, p[y].w[u], o[y][cb]);
                 }
         }
     }
 
-    // 32 keys that stand in LDS at kt, vt.  seen: bit j = this lane's query sees key j; all: every query of the wave sees every key;
-    // odd: bit j = key j's values were not all finite (take_odd)
-    __device__ __forceinline__ void block(uint32_t kt, uint32_t vt, uint32_t seen, bool all, uint32_t odd) {
-        f32x16 s[MAPS];
+    // 32 keys that stand in LDS at kt, vt.  bits: those that somebody may see; rest: how many of them at most this lane's query sees (its causal end or length);
+    // all: every query of the wave sees every key; odd: bit j = key j's values were not all finite (take_odd)
+    __device__ __forceinline__ void block(uint32_t kt, uint32_t vt, uint32_t bits, int rest, bool all, uint32_t odd) {
+        Weights<T> p[MAPS];
         float t[MAPS];
-        const uint32_t mine = seen >> (4 * h);
+        auto mine = [&] { return (bits & (uint32_t)below(rest)) >> (4 * h); };
         bool done = false, fine = true;
-        if (started) done = all ? straight<false>(kt, mine, s, t, fine) : straight<true>(kt, mine, s, t, fine);
+        if (started) done = all ? straight<false>(kt, 0, p, t, fine) : straight<true>(kt, mine(), p, t, fine);
         if (!done) {
             // Hardly ever taken: one map after the other, on fragments read anew.  What the path above holds is not kept for this one (registers).  A row is centred
             // anew for its own sake alone: its result does not depend on the rows beside it.
@@ -303,10 +325,10 @@ template <typename T, int D, int MAPS> struct Wave {
 #pragma unroll
                 for (int y = 0; y < MAPS; ++y) {
                     __builtin_amdgcn_sched_barrier(0);
-                    s[y] = scores(again, y);
-                    recentre(s[y], y, mine, need);
-                    exponentials(s[y], m[y] == -INFINITY ? 0.f : m[y]);
-                    t[y] = sum(s[y]);
+                    f32x16 s = scores(again, y);
+                    recentre(s, y, mine(), need);
+                    exponentials(s, m[y] == -INFINITY ? 0.f : m[y]);
+                    t[y] = p[y].set(s);
                     over = over || !(t[y] <= kMost);
                     started = started && __all(m[y] > -INFINITY);
                 }
@@ -316,15 +338,12 @@ template <typename T, int D, int MAPS> struct Wave {
                 need = need || over;
             }
         }
-        const float poison = seen & odd ? __builtin_nanf("") : 0.f;
+        if (odd && mine() & odd >> (4 * h)) t[0] = __builtin_nanf("");
 #pragma unroll
-        for (int y = 0; y < MAPS; ++y) l[y] += t[y] + poison;
-        values(vt, s);
+        for (int y = 0; y < MAPS; ++y) l[y] += t[y];
+        values(vt, p);
     }
 };
-
-// bits of the keys below `n` (any n)
-__device__ __forceinline__ uint64_t below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // LDS-DMA of 16 bytes per lane to 1 KB at `lds` (wave-uniform), from a uniform address plus a lane's offset, or from a lane's address.  Written in assembly: the
 // compiler takes every LDS read behind its own builtin to depend on the copy and would wait for the next tile before it reads this one.  The copies have no
@@ -439,7 +458,7 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     const int row0 = at.rb * F::BR + 32 * group;
 
     int n = a.n_k;
-    if (a.kv_lens_dev) n = min(max(a.kv_lens_dev[at.b], 0), n);
+    if (a.kv_lens_dev) n = min(max(__builtin_amdgcn_readfirstlane(a.kv_lens_dev[at.b]), 0), n);
     const int shift = a.causal == RZ_CAUSAL_END ? n - a.n_q : 0;
     auto limit = [&](int query) { return a.causal ? min(n, query + 1 + shift) : n; };       // keys that a query may see at most (may be negative)
     int lim;
@@ -516,6 +535,7 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     for (int y = 0; y < MAPS; ++y)
 #pragma unroll
         for (int t = 0; t < S::NT; ++t) asm volatile("" : "+v"(wv.q[y][t]));
+    const uint32_t k_at = Wave<T, D, MAPS>::k_lane(lane) + map * (S::RB / 2), v_at = TILE + Wave<T, D, MAPS>::v_lane(lane);
     find();
     if (bits_next) fill(mine, j_first + k_next * STEP, bits_next);
     int turn = 0;
@@ -540,12 +560,10 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
                 else __syncthreads();
             }
         }
-        const int again = fresh(lane);
-        const uint32_t kt = lds_address(buf) + Wave<T, D, MAPS>::k_lane(again) + map * (S::RB / 2), vt = lds_address(buf) + TILE + Wave<T, D, MAPS>::v_lane(again);
+        const uint32_t kt = lds_address(buf) + k_at, vt = lds_address(buf) + v_at;
 #pragma unroll
         for (int kb = 0; kb < BN / 32; ++kb) {
-            const uint32_t seen = (uint32_t)((bits & below(lim - j)) >> (32 * kb));
-            wv.block(kt + kb * 32 * S::RB, vt + kb * 32 * S::RB, seen, all, (uint32_t)(odd >> (32 * kb)));
+            wv.block(kt + kb * 32 * S::RB, vt + kb * 32 * S::RB, (uint32_t)(bits >> (32 * kb)), lim - j - 32 * kb, all, (uint32_t)(odd >> (32 * kb)));
         }
         turn ^= 1;
     }

@@ -40,6 +40,7 @@ def _need(ok, what):
 
 
 def _tokens(x, name, dim, like=None):
+    """Says what is wrong with a tensor of tokens."""
     _need(isinstance(x, torch.Tensor) and x.dim() == dim, f"{name} must be a tensor of {dim} dimensions")
     _need(x.is_cuda, f"{name} must be on the GPU (there is no CPU fallback)")
     _need(x.dtype in _DTYPES, f"{name} must be float32, bfloat16 or float16")
@@ -51,12 +52,13 @@ def _tokens(x, name, dim, like=None):
 
 
 def _vector(x, name, shape, device):
-    """Data pointer of a contiguous float32 tensor, None for None."""
+    """Address of a contiguous float32 tensor, 0 for None."""
     if x is None:
-        return None
-    _need(isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.shape == shape, f"{name} must be float32 {tuple(shape)}")
-    _need(x.device == device and x.is_contiguous(), f"{name} must be contiguous on {device}")
-    _need(not (x.requires_grad and torch.is_grad_enabled()), f"{name} asks for a gradient: these operators are forward only (torch.no_grad())")
+        return 0
+    if not (isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.shape == shape and x.device == device and x.is_contiguous() and not x.requires_grad):
+        _need(isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.shape == shape, f"{name} must be float32 {tuple(shape)}")
+        _need(x.device == device and x.is_contiguous(), f"{name} must be contiguous on {device}")
+        _need(not torch.is_grad_enabled(), f"{name} asks for a gradient: these operators are forward only (torch.no_grad())")
     return x.data_ptr()
 
 
@@ -69,12 +71,31 @@ def _output(out, like_shape, dtype, device, name):
     return out
 
 
-def _call(fn, device, *args):
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), fn.__name__)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_entry = {}
+
+
+def _fn(name, *argtypes):
+    """An entry point that takes its struct as bytes (the prototypes in _lib.SYMBOLS take the ctypes mirrors)."""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = ctypes.CFUNCTYPE(_lib.SYMBOLS[name][0], ctypes.c_char_p, *argtypes)((name, _lib.load()))
+    return fn
+
+
+def _call(name, argtypes, device, *args):
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = _fn(name, *argtypes)(*args, _raw_stream(index))
     else:                                                # kernels go to the tensors' device, on its current stream
         with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream().cuda_stream), fn.__name__)
+            rc = _fn(name, *argtypes)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+_STREAM = (ctypes.c_void_p,)
+_WORKSPACE_STREAM = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p)
 
 
 def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, axes: int = 1, scaling: Optional[dict] = None, device=None) -> Tuple[torch.Tensor, float]:
@@ -122,43 +143,41 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torc
     positions: int64, (tokens,) or (batch, tokens), with a last dimension of `axes` if freqs has two dimensions; |position| < 2^31.
     layout: "half" pairs column p with p + rotary_dim / 2, "interleaved" 2 p with 2 p + 1.
     out: tensors to write (q_out, or (q_out, k_out)); the inputs themselves are fine.  Returns q_out, or (q_out, k_out) with k."""
-    _tokens(q, "q", 4)
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES and q.dim() == 4 and q.stride(3) == 1 and not q.requires_grad):
+        _tokens(q, "q", 4)
     b, n, hq, d = q.shape
-    dev = q.device
-    hk = 0
+    dev, dt = q.device, q.dtype
+    hk, ks = 0, (0, 0, 0)
     if k is not None:
-        _tokens(k, "k", 4, q)
-        hk = k.shape[2]
-        _need(k.shape[0] == b and k.shape[1] == n and k.shape[3] == d, "q and k must agree in batch, tokens and head_dim")
+        if not (isinstance(k, torch.Tensor) and k.dtype is dt and k.device == dev and k.dim() == 4 and k.stride(3) == 1 and not k.requires_grad):
+            _tokens(k, "k", 4, q)
+        kb, kn, hk, kd = k.shape
+        _need(kb == b and kn == n and kd == d, "q and k must agree in batch, tokens and head_dim")
     _need(layout in _LAYOUT, "layout must be half or interleaved")
-    _need(isinstance(freqs, torch.Tensor) and freqs.dtype == torch.float64 and freqs.dim() in (1, 2) and freqs.device == dev and freqs.is_contiguous(),
-          f"freqs must be contiguous float64 (pairs,) or (axes, pairs) on {dev}")
-    axes = freqs.shape[0] if freqs.dim() == 2 else 1
+    _need(isinstance(freqs, torch.Tensor) and freqs.dtype is torch.float64 and freqs.dim() in (1, 2) and freqs.device == dev and freqs.is_contiguous(),
+          "freqs must be contiguous float64 (pairs,) or (axes, pairs) on q's device")
     pos = positions
-    _need(isinstance(pos, torch.Tensor) and pos.dtype == torch.int64 and pos.device == dev, f"positions must be int64 on {dev}")
+    _need(isinstance(pos, torch.Tensor) and pos.dtype is torch.int64 and pos.device == dev, "positions must be int64 on q's device")
+    shape, strides, axes = tuple(pos.shape), pos.stride(), 1
     if freqs.dim() == 2:
-        _need(pos.dim() in (2, 3) and pos.shape[-1] == axes and (pos.stride(-1) == 1 or axes == 1), "positions need a contiguous last dimension of one value per axis")
-        shape, strides = pos.shape[:-1], pos.stride()[:-1]
-    else:
-        shape, strides = pos.shape, pos.stride()
-    _need(tuple(shape) in ((n,), (b, n)), "positions must be (tokens,) or (batch, tokens)")
+        axes = freqs.shape[0]
+        _need(len(shape) in (2, 3) and shape[-1] == axes and (strides[-1] == 1 or axes == 1), "positions need a contiguous last dimension of one value per axis")
+        shape, strides = shape[:-1], strides[:-1]
+    _need(shape == (b, n) or shape == (n,), "positions must be (tokens,) or (batch, tokens)")
     if out is None:
-        qo = torch.empty((b, n, hq, d), dtype=q.dtype, device=dev)
-        ko = torch.empty((b, n, hk, d), dtype=q.dtype, device=dev) if k is not None else None
+        qo = torch.empty((b, n, hq, d), dtype=dt, device=dev)
+        ko = torch.empty((b, n, hk, d), dtype=dt, device=dev) if k is not None else None
     else:
         qo, ko = (out, None) if k is None else out
-        qo = _output(qo, q.shape, q.dtype, dev, "out")
-        ko = None if k is None else _output(ko, k.shape, q.dtype, dev, "out")
+        qo = _output(qo, q.shape, dt, dev, "out")
+        ko = None if k is None else _output(ko, k.shape, dt, dev, "out")
+    kos, kp, kop = ks, 0, 0
     if hk:
         ks, kos, kp, kop = k.stride(), ko.stride(), k.data_ptr(), ko.data_ptr()
-    else:
-        ks = kos = (0, 0, 0)
-        kp = kop = None
     qs, qos = q.stride(), qo.stride()
-    a = _lib.RzRotaryArgs(_DTYPES[q.dtype], _LAYOUT[layout], b, n, hq, hk, d, 2 * freqs.numel(), axes, amplitude, q.data_ptr(), qs[0], qs[1], qs[2],
-                          kp, ks[0], ks[1], ks[2], qo.data_ptr(), qos[0], qos[1], qos[2], kop, kos[0], kos[1], kos[2],
-                          pos.data_ptr(), strides[0] if len(shape) == 2 else 0, strides[-1], freqs.data_ptr())
-    _call(_lib.load().rz_rotary, dev, ctypes.byref(a))
+    _call("rz_rotary", _STREAM, dev, _lib.RzRotaryArgs.pack(
+        _DTYPES[dt], _LAYOUT[layout], b, n, hq, hk, d, 2 * freqs.numel(), axes, amplitude, q.data_ptr(), qs[0], qs[1], qs[2], kp, ks[0], ks[1], ks[2],
+        qo.data_ptr(), qos[0], qos[1], qos[2], kop, kos[0], kos[1], kos[2], pos.data_ptr(), strides[0] if len(shape) == 2 else 0, strides[-1], freqs.data_ptr()))
     return qo if k is None else (qo, ko)
 
 
@@ -173,43 +192,49 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
     kv_lens integer (batch,): only the first kv_lens[b] keys count.  attention_mask (batch, n_k): 0 = hidden, as a tokenizer gives it.  A query that sees
     no key gets zeros; what hidden keys hold changes nothing.  norm_weight float32 (2 d): root-mean-square norm of every head's output.
     16-byte alignment of q, k, v and out and of their strides is required.  Returns (batch, n_q, heads, 2 d), in `out` (no input's memory) if given."""
-    _tokens(q, "q", 4)
-    _tokens(k, "k", 4, q)
-    _tokens(v, "v", 4, q)
-    b, n_q, h, w = q.shape
-    n_k, hk = k.shape[1], k.shape[2]
-    dev = q.device
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES and q.dim() == 4 and not q.requires_grad):
+        _tokens(q, "q", 4)
+    dev, dt = q.device, q.dtype
+    for x, name in ((k, "k"), (v, "v")):
+        if not (isinstance(x, torch.Tensor) and x.dtype is dt and x.device == dev and x.dim() == 4 and not x.requires_grad):
+            _tokens(x, name, 4, q)
+    (b, n_q, h, w), (kb, n_k, hk, kw) = q.shape, k.shape
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
     d = w // 2
     _need(w in (64, 128, 256), "the last dimension must be 64, 128 or 256 (two maps of 32, 64 or 128)")
-    _need(k.shape == v.shape and k.shape[0] == b and k.shape[3] == w, "k and v must be (batch, n_k, kv_heads, 2 d), like q in batch and 2 d")
+    _need(kb == b and kw == w and v.shape == k.shape, "k and v must be (batch, n_k, kv_heads, 2 d), like q in batch and 2 d")
+    _need(qs[3] == 1 and ks[3] == 1 and vs[3] == 1, "q, k, v: columns must be contiguous")
     _need(h >= 1 and hk >= 1, "there must be a head of q and of k")
     _need(causal in _CAUSAL, "causal must be None, start or end")
     per_head = isinstance(lambda_qk, torch.Tensor) and lambda_qk.dim() == 3
     lam = _vector(lambda_qk, "lambda_qk", (h, 4, d) if per_head else (4, d), dev)
-    _need(lam is not None, "lambda_qk must be a tensor")
+    _need(lam, "lambda_qk must be a tensor")
+    lens = 0
     if kv_lens is not None:
         _need(isinstance(kv_lens, torch.Tensor) and kv_lens.shape == (b,) and kv_lens.device == dev and kv_lens.dtype in (torch.int32, torch.int64),
-              f"kv_lens must be int32 or int64 (batch,) on {dev}")
-        if kv_lens.dtype == torch.int64:
+              "kv_lens must be int32 or int64 (batch,) on q's device")
+        if kv_lens.dtype is torch.int64:
             kv_lens = kv_lens.clamp(0, n_k).to(torch.int32)
         kv_lens = kv_lens.contiguous()
-    mask = attention_mask
-    if mask is not None:
-        _need(isinstance(mask, torch.Tensor) and mask.shape == (b, n_k) and mask.device == dev and not mask.dtype.is_floating_point and not mask.dtype.is_complex,
-              f"attention_mask must be integer or bool (batch, n_k) on {dev}")
-        mask = mask.to(torch.int64)
-        if n_k > 1 and mask.stride(1) != 1:
-            mask = mask.contiguous()
-    out = _output(out, q.shape, q.dtype, dev, "out")
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-    a = _lib.RzDiffAttentionArgs(_DTYPES[q.dtype], b, h, hk, n_q, n_k, d, _CAUSAL[causal], d ** -0.5 if scale is None else scale, lambda_init, norm_eps, out_scale,
-                                 q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-                                 out.data_ptr(), os[0], os[1], os[2], lam, 4 * d if per_head else 0, _vector(norm_weight, "norm_weight", (w,), dev),
-                                 None if kv_lens is None else kv_lens.data_ptr(), None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0))
-    lib, ref = _lib.load(), ctypes.byref(a)
-    need = lib.rz_diff_attention_workspace(ref)
+        lens = kv_lens.data_ptr()
+    mask, mask_stride = 0, 0
+    if attention_mask is not None:
+        x = attention_mask
+        _need(isinstance(x, torch.Tensor) and x.shape == (b, n_k) and x.device == dev and not x.dtype.is_floating_point and not x.dtype.is_complex,
+              "attention_mask must be integer or bool (batch, n_k) on q's device")
+        x = x.to(torch.int64)
+        if n_k > 1 and x.stride(1) != 1:
+            x = x.contiguous()
+        attention_mask, mask, mask_stride = x, x.data_ptr(), x.stride(0)
+    out = torch.empty((b, n_q, h, w), dtype=dt, device=dev) if out is None else _output(out, q.shape, dt, dev, "out")
+    os = out.stride()
+    args = _lib.RzDiffAttentionArgs.pack(
+        _DTYPES[dt], b, h, hk, n_q, n_k, d, _CAUSAL[causal], d ** -0.5 if scale is None else scale, lambda_init, norm_eps, out_scale,
+        q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], out.data_ptr(), os[0], os[1], os[2],
+        lam, 4 * d if per_head else 0, _vector(norm_weight, "norm_weight", (w,), dev), lens, mask, mask_stride)
+    need = _fn("rz_diff_attention_workspace")(args)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(lib.rz_diff_attention, dev, ref, None if ws is None else ws.data_ptr(), need)
+    _call("rz_diff_attention", _WORKSPACE_STREAM, dev, args, ws.data_ptr() if need else 0, need)
     return out
 
 
@@ -223,47 +248,57 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
     x has y's type (without y: `dtype`, else the residual's).  pre_norm None: x is None.  out: (r, x) to write; r may be `residual`, x may be `y`.
     pre_norm's statistics are those of r in float32, before it is rounded to the residual's type."""
     nd = residual.dim() if isinstance(residual, torch.Tensor) else 0
-    _need(nd in (2, 3), "residual must be (rows, dim) or (batch, rows, dim)")
-    _tokens(residual, "residual", nd)
-    dev, shape, dim = residual.device, residual.shape, residual.shape[-1]
-    t = dtype if dtype is not None else residual.dtype
+    _need(nd == 2 or nd == 3, "residual must be (rows, dim) or (batch, rows, dim)")
+    hs = residual.stride()
+    if not (residual.is_cuda and residual.dtype in _DTYPES and hs[-1] == 1 and not residual.requires_grad):
+        _tokens(residual, "residual", nd)
+    dev, rt, shape = residual.device, residual.dtype, residual.shape
+    dim = shape[-1]
+    t = rt if dtype is None else dtype
+    yp, ys = 0, (0, 0, 0)
     if y is not None:
-        _tokens(y, "y", nd)
+        if not (isinstance(y, torch.Tensor) and y.dtype in _DTYPES and y.device == dev and y.dim() == nd and y.stride(-1) == 1 and not y.requires_grad):
+            _tokens(y, "y", nd)
         _need(y.shape == shape and y.device == dev, "y must have the residual's shape and device")
-        _need(dtype is None or dtype == y.dtype, "x has y's type")
-        t = y.dtype
-    _need(t in _DTYPES and (residual.dtype == torch.float32 or residual.dtype == t), "the residual must be float32 or of x's type")
-    _need(y is not None or (post_norm is None and scale is None and gate is None), "post_norm, scale and gate need y")
-    gs = (0, 0)
+        _need(dtype is None or dtype is y.dtype, "x has y's type")
+        t, yp, ys = y.dtype, y.data_ptr(), y.stride()
+    else:
+        _need(post_norm is None and scale is None and gate is None, "post_norm, scale and gate need y")
+    _need(t in _DTYPES and (rt is torch.float32 or rt is t), "the residual must be float32 or of x's type")
+    gp, gb, gr = 0, 0, 0
     if gate is not None:
-        _need(isinstance(gate, torch.Tensor) and gate.dtype == torch.float32 and gate.device == dev and 1 <= gate.dim() <= nd, f"gate must be float32 on {dev}")
+        _need(isinstance(gate, torch.Tensor) and gate.dtype is torch.float32 and gate.device == dev and 1 <= gate.dim() <= nd, "gate must be float32 on the residual's device")
         full = (dim,) if gate.dim() == 1 else shape if gate.dim() == nd else (shape[0], dim)
         _need(tuple(gate.shape) == tuple(full) and (gate.stride(-1) == 1 or dim == 1), "gate must be (dim,), (batch, dim) or the residual's shape, columns contiguous")
         _need(not (gate.requires_grad and torch.is_grad_enabled()), "gate asks for a gradient: these operators are forward only (torch.no_grad())")
         st = gate.stride()
-        gs = (0, 0) if gate.dim() == 1 else (st[0], st[1]) if gate.dim() == 3 else (st[0], 0) if nd == 3 else (0, st[0])
+        gp = gate.data_ptr()
+        gb, gr = (0, 0) if gate.dim() == 1 else (st[0], st[1]) if gate.dim() == 3 else (st[0], 0) if nd == 3 else (0, st[0])
     ro, xo = (None, None) if out is None else out
-    write_r = y is not None or alpha != 1.0 or ro is not None or pre_norm is None
-    ro = _output(ro, shape, residual.dtype, dev, "out[0]") if write_r else residual
-    _need(xo is None or pre_norm is not None, "out[1] needs pre_norm")
-    xo = _output(xo, shape, t, dev, "out[1]") if pre_norm is not None else None
-
-    def rows(x):
-        if x is None:
-            return 0, 0
-        st = x.stride()
-        return (st[0], st[1]) if nd == 3 else (0, st[0])
-
-    def norm(x, name):
-        if x is None:
-            return 0, 0.0, None, None
-        _need(x.kind in _NORM, f"{name}.kind must be layer or rms")
-        return _NORM[x.kind], x.eps, _vector(x.weight, f"{name}.weight", (dim,), dev), _vector(x.bias, f"{name}.bias", (dim,), dev)
-
-    post, pre = norm(post_norm, "post_norm"), norm(pre_norm, "pre_norm")
-    a = _lib.RzResidualNormArgs(_DTYPES[t], _DTYPES[residual.dtype], shape[0] if nd == 3 else 1, shape[-2], dim, post[0], pre[0], alpha, post[1], pre[1],
-                                None if y is None else y.data_ptr(), *rows(y), residual.data_ptr(), *rows(residual),
-                                ro.data_ptr() if write_r else None, *rows(ro), None if xo is None else xo.data_ptr(), *rows(xo),
-                                post[2], post[3], _vector(scale, "scale", (dim,), dev), None if gate is None else gate.data_ptr(), *gs, pre[2], pre[3])
-    _call(_lib.load().rz_residual_norm, dev, ctypes.byref(a))
+    rp, rs, xp, xs = 0, (0, 0, 0), 0, (0, 0, 0)
+    if y is not None or alpha != 1.0 or ro is not None or pre_norm is None:
+        ro = torch.empty(shape, dtype=rt, device=dev) if ro is None else _output(ro, shape, rt, dev, "out[0]")
+        rp, rs = ro.data_ptr(), ro.stride()
+    else:
+        ro = residual
+    post_kind, post_eps, post_w, post_b, pre_kind, pre_eps, pre_w, pre_b = 0, 0.0, 0, 0, 0, 0.0, 0, 0
+    if post_norm is not None:
+        post_w, post_b, post_eps, post_kind = post_norm
+        _need(post_kind in _NORM, "post_norm.kind must be layer or rms")
+        post_kind, post_w, post_b = _NORM[post_kind], _vector(post_w, "post_norm.weight", (dim,), dev), _vector(post_b, "post_norm.bias", (dim,), dev)
+    if pre_norm is not None:
+        pre_w, pre_b, pre_eps, pre_kind = pre_norm
+        _need(pre_kind in _NORM, "pre_norm.kind must be layer or rms")
+        pre_kind, pre_w, pre_b = _NORM[pre_kind], _vector(pre_w, "pre_norm.weight", (dim,), dev), _vector(pre_b, "pre_norm.bias", (dim,), dev)
+        xo = torch.empty(shape, dtype=t, device=dev) if xo is None else _output(xo, shape, t, dev, "out[1]")
+        xp, xs = xo.data_ptr(), xo.stride()
+    else:
+        _need(xo is None, "out[1] needs pre_norm")
+    if nd == 2:
+        batch, rows, hs, ys, rs, xs = 1, shape[0], (0, *hs), (0, *ys), (0, *rs), (0, *xs)
+    else:
+        batch, rows = shape[0], shape[1]
+    _call("rz_residual_norm", _STREAM, dev, _lib.RzResidualNormArgs.pack(
+        _DTYPES[t], _DTYPES[rt], batch, rows, dim, post_kind, pre_kind, alpha, post_eps, pre_eps, yp, ys[0], ys[1], residual.data_ptr(), hs[0], hs[1], rp, rs[0], rs[1],
+        xp, xs[0], xs[1], post_w, post_b, _vector(scale, "scale", (dim,), dev), gp, gb, gr, pre_w, pre_b))
     return ro, xo

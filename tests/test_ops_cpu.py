@@ -114,6 +114,17 @@ def test_structs_have_the_size_the_compiler_gives_them(tmp_path):
     assert got == [ctypes.sizeof(t) for _, t in pairs] + [getattr(t, n).offset for _, t in pairs for n, _ in t._fields_]
 
 
+def test_packed_structs_are_the_ctypes_ones():
+    for t in (_lib.RzRotaryArgs, _lib.RzDiffAttentionArgs, _lib.RzResidualNormArgs):
+        a, values = t(), []
+        for i, (n, c) in enumerate(t._fields_):
+            values.append(i + 0.5 if c is ctypes.c_float else i + 1)
+            setattr(a, n, values[-1])
+        packed = t.pack(*values)
+        assert packed == bytes(a)[:len(packed)] and not any(bytes(a)[len(packed):])
+        assert (ctypes.c_char * len(packed)).from_buffer_copy(packed).raw == packed
+
+
 def test_rotary_frequencies():
     f, a = ops.rotary_frequencies(8, base=100.0)
     assert f.dtype == torch.float64 and a == 1.0
