@@ -135,20 +135,24 @@ struct Args {
     rz_diff_attention_args a;
     int group, rows, row_blocks;                               // heads per key head, query rows per key head, their blocks
     int units, full, splits;
+    float c;                                                   // scale * log2(e)
     int part_rows;                                             // rows of a unit in the workspace
     float* ws;
 };
 // workspace, floats: [unit - full][split][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
 __host__ __device__ inline int64_t parts(const Args& x) { return (int64_t)(x.units - x.full) * x.splits * x.part_rows; }
 
+// a value that is the same in all lanes, into a scalar register (divisions run on the vector unit)
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 struct Work {
     int unit, split, rb, hk, b;
     bool whole;
     __device__ __forceinline__ void place(const Args& x) {
-        rb = x.row_blocks - 1 - unit % x.row_blocks;           // row blocks innermost: they read the same keys; causal: the longest first
-        const int bh = unit / x.row_blocks;
-        hk = bh % x.a.kv_heads;
-        b = bh / x.a.kv_heads;
+        rb = x.row_blocks - 1 - scalar(unit % x.row_blocks);   // row blocks innermost: they read the same keys; causal: the longest first
+        const int bh = scalar(unit / x.row_blocks);
+        hk = scalar(bh % x.a.kv_heads);
+        b = scalar(bh / x.a.kv_heads);
     }
     __device__ __forceinline__ Work(const Args& x) {
         const int id = blockIdx.x;
@@ -156,8 +160,8 @@ struct Work {
         if (whole) unit = xcd_remap(id, x.full), split = 0;
         else {
             const int t = xcd_remap(id - x.full, gridDim.x - x.full);
-            unit = x.full + t / x.splits;
-            split = t % x.splits;
+            unit = x.full + scalar(t / x.splits);
+            split = scalar(t % x.splits);
             whole = x.splits == 1;
         }
         place(x);
@@ -193,7 +197,7 @@ template <typename T, int D, int MAPS> struct Wave {
     bool started;                     // every row has a reference maximum (wave-uniform)
 
     __device__ __forceinline__ void init(const Args& x, const T* qrow) {      // qrow: the first of the wave's maps
-        c = x.a.scale * 1.44269504088896340736f;
+        c = x.c;
         started = false;
 #pragma unroll
         for (int y = 0; y < MAPS; ++y) {
@@ -359,31 +363,41 @@ __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0) lgkm
 
 // Fills LDS rows [0, ROWS) x RB bytes with keys j0 ..; wave w of W.  Keys that nobody may see (bits 0: hidden, or behind the last) are replaced by the first that
 // somebody does: their weights are 0, and 0 * (what a hidden place holds) would not be.
-template <typename T, int D, int ROWS, int W, bool VALUES>
-__device__ __forceinline__ void stage(char* lds, const char* src, int64_t stride, int j0, uint64_t bits, int w, int lane) {
+template <typename T, int D, int ROWS, int W, bool VALUES> struct Stage {
     typedef Shape<T, D> S;
-    constexpr int per = 1024 / S::RB, N = ROWS * S::RB / 1024 / W;         // rows of one LDS-DMA instruction (1 KB), instructions of a wave
+    static constexpr int per = 1024 / S::RB, N = ROWS * S::RB / 1024 / W;  // rows of one LDS-DMA instruction (1 KB), instructions of a wave
     static_assert(S::RB <= 1024 && ROWS * S::RB % (1024 * W) == 0, "tile and waves do not fit");
-    lane = fresh(lane);
-    const int sub = lane / S::CH, cp = lane % S::CH;
-    if (bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1)) {        // every key: a uniform address and a lane's offset that is the same in every tile
-        const uint32_t in = (uint32_t)sub * (uint32_t)stride;
-        const char* base = src + (int64_t)j0 * stride;
+    const char* src;
+    int64_t stride;
+    int w;
+    uint32_t in;                                                           // a lane's row, from the first of its instruction
+    static __device__ __forceinline__ int swz(int r) { return VALUES ? S::swz_v(r) : S::swz_k(r); }
+
+    __device__ __forceinline__ void init(const void* p, int64_t bytes, int wave, int lane) {
+        src = (const char*)p, stride = bytes, w = wave;
+        in = (uint32_t)(lane / S::CH) * (uint32_t)stride;
+    }
+    __device__ __forceinline__ void fill(char* lds, int j0, uint64_t bits, int lane) const {
+        lane = fresh(lane);
+        const int sub = lane / S::CH, cp = lane % S::CH ^ swz(sub);        // a row's XOR is that of its instruction's first row and its own place behind it
+        if (bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1)) {    // every key: a uniform address and a lane's offset
+            const char* base = src + (j0 + w * N * per) * stride;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int r0 = (w * N + i) * per, r = r0 + sub;
-            lds_dma(lds + r0 * S::RB, base + (int64_t)r0 * stride, in + ((cp ^ (VALUES ? S::swz_v(r) : S::swz_k(r))) << 4));
-        }
-    } else {
-        const int first = __builtin_ctzll(bits);
+            for (int i = 0; i < N; ++i, base += per * stride) {
+                const int r0 = (w * N + i) * per;
+                lds_dma(lds + r0 * S::RB, base, in + ((cp ^ swz(r0)) << 4));
+            }
+        } else {
+            const int first = __builtin_ctzll(bits);
 #pragma unroll 1
-        for (int i = 0; i < N; ++i) {
-            const int r0 = (w * N + i) * per, r = r0 + sub;
-            const int key = j0 + ((bits >> r) & 1 ? r : first);
-            lds_dma(lds + r0 * S::RB, src + (int64_t)key * stride + ((cp ^ (VALUES ? S::swz_v(r) : S::swz_k(r))) << 4));
+            for (int i = 0; i < N; ++i) {
+                const int r0 = (w * N + i) * per, r = r0 + sub;
+                const int key = j0 + ((bits >> r) & 1 ? r : first);
+                lds_dma(lds + r0 * S::RB, src + (int64_t)key * stride + ((cp ^ swz(r0)) << 4));
+            }
         }
     }
-}
+};
 
 // Values that are not finite, in a tile that not every query sees in full (causal): 0 * inf is not 0, so they would reach queries that must not see them.
 // Returns the keys (bits) that hold any; take_odd then clears those values in LDS, and a query that does see such a key becomes NaN through its sum.
@@ -399,11 +413,14 @@ template <typename T, int D, int ROWS> __device__ __forceinline__ uint64_t odd_k
     typedef Shape<T, D> S;
     constexpr int N = ROWS * S::RB / 1024, per = 64 / S::CH;
     bool any = false;
+#pragma unroll 4
     for (int n = 0; n < N; ++n) any |= odd_chunk<T>(*reinterpret_cast<const u32x4*>(vt + (n * 64 + lane) * 16));
     uint64_t keys = 0;
     if (__any(any))
+#pragma unroll 1
         for (int n = 0; n < N; ++n) {
             const uint64_t b = __ballot(odd_chunk<T>(*reinterpret_cast<const u32x4*>(vt + (n * 64 + lane) * 16)));
+#pragma unroll 1
             for (int r = 0; r < per; ++r)
                 if (b >> (r * S::CH) & (S::CH == 64 ? ~0ull : (1ull << (S::CH & 63)) - 1)) keys |= 1ull << (n * per + r);
         }
@@ -411,6 +428,7 @@ template <typename T, int D, int ROWS> __device__ __forceinline__ uint64_t odd_k
 }
 template <typename T, int D, int ROWS> __device__ __forceinline__ void take_odd(char* vt, int lane) {
     constexpr int N = ROWS * Shape<T, D>::RB / (64 * (int)sizeof(T));
+#pragma unroll 1
     for (int n = 0; n < N; ++n) {
         T* v = (T*)vt + n * 64 + lane;
         if (!(fabsf(to_f32(*v)) < INFINITY)) *v = (T)0.f;
@@ -458,17 +476,17 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     const int row0 = at.rb * F::BR + 32 * group;
 
     int n = a.n_k;
-    if (a.kv_lens_dev) n = min(max(__builtin_amdgcn_readfirstlane(a.kv_lens_dev[at.b]), 0), n);
+    if (a.kv_lens_dev) n = min(max(scalar(a.kv_lens_dev[at.b]), 0), n);
     const int shift = a.causal == RZ_CAUSAL_END ? n - a.n_q : 0;
-    auto limit = [&](int query) { return a.causal ? min(n, query + 1 + shift) : n; };       // keys that a query may see at most (may be negative)
+    auto limit = [&](int query) -> int { return a.causal ? min(n, query + 1 + shift) : n; };       // keys that a query may see at most (may be negative)
     int lim;
     const int last = min((at.rb + 1) * F::BR, x.rows) - 1;
-    const int end = max(limit(last / x.group), 0);                         // of the workgroup
-    const int wave_first = limit(min(row0, x.rows - 1) / x.group);         // keys that every query of the wave sees, but for hidden ones
-    const int unit_first = limit(at.rb * F::BR / x.group);                 // the same of the workgroup
+    const int end = max(limit(scalar(last / x.group)), 0);                         // of the workgroup
+    const int wave_first = limit(scalar(min(row0, x.rows - 1) / x.group));         // keys that every query of the wave sees, but for hidden ones
+    const int unit_first = limit(scalar(at.rb * F::BR / x.group));                 // the same of the workgroup
     int begin = 0, stop = end;
     if (!at.whole) {
-        const int per = ((end + x.splits - 1) / x.splits + 63) / 64 * 64;
+        const int per = scalar(((end + x.splits - 1) / x.splits + 63) / 64 * 64);
         begin = min(at.split * per, end);
         stop = min(begin + per, end);
     }
@@ -481,9 +499,10 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
         wv.init(x, (const T*)a.q_dev + at.b * a.q_batch_stride + i * a.q_token_stride + head * a.q_head_stride + map * D);
     }
 
-    const char* kp = (const char*)((const T*)a.k_dev + at.b * a.k_batch_stride + at.hk * a.k_head_stride);
-    const char* vp = (const char*)((const T*)a.v_dev + at.b * a.v_batch_stride + at.hk * a.v_head_stride);
-    const int64_t ks = a.k_token_stride * (int64_t)sizeof(T), vs = a.v_token_stride * (int64_t)sizeof(T);
+    Stage<T, D, BN, KEYS ? 1 : W, false> keys;
+    Stage<T, D, BN, KEYS ? 1 : W, true> values;
+    keys.init((const T*)a.k_dev + at.b * a.k_batch_stride + at.hk * a.k_head_stride, a.k_token_stride * (int64_t)sizeof(T), KEYS ? 0 : wave, lane);
+    values.init((const T*)a.v_dev + at.b * a.v_batch_stride + at.hk * a.v_head_stride, a.v_token_stride * (int64_t)sizeof(T), KEYS ? 0 : wave, lane);
     const int64_t* mask = a.mask_dev ? a.mask_dev + at.b * a.mask_batch_stride : nullptr;
     constexpr int STEP = KEYS ? BN * W : BN;
     const int j_first = begin + (KEYS ? wave * BN : 0);
@@ -526,8 +545,8 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
         }
     };
     auto fill = [&](char* buf, int j, uint64_t bits) {
-        stage<T, D, BN, KEYS ? 1 : W, false>(buf, kp, ks, j, bits, KEYS ? 0 : wave, lane);
-        stage<T, D, BN, KEYS ? 1 : W, true>(buf + TILE, vp, vs, j, bits, KEYS ? 0 : wave, lane);
+        keys.fill(buf, j, bits, lane);
+        values.fill(buf + TILE, j, bits, lane);
     };
     char* mine = lds + (KEYS ? wave * 2 * BUF : 0);
     // the queries are there before the first copy leaves: a wait for them inside the loop would be one for the copies too
@@ -758,6 +777,7 @@ template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& 
     typedef Form<T, D, KEYS> F;
     Args x;
     x.a = a;
+    x.c = a.scale * 1.44269504088896340736f;
     x.group = a.heads / a.kv_heads;
     x.rows = a.n_q * x.group;
     x.row_blocks = (x.rows + F::BR - 1) / F::BR;
