@@ -393,6 +393,24 @@ def test_residual_norm_views_in_place_and_neighbours(ops, dtype):
     assert r.shape == (b, 0, d) and x.shape == (b, 0, d)
 
 
+@pytest.mark.parametrize("d", [64, 190, 768, 1024], ids=str)
+def test_residual_norm_many_rows(ops, d):
+    """More rows than waves, so that a wave takes several, with runs that cross from one sample to the next: each sample's own gate, a gate per row, in place."""
+    g = gen(35 + d)
+    b, n = 5, 2741
+    residual, y = randn(g, b, n, d), randn(g, b, n, d, dtype=torch.bfloat16)
+    pre, post, scale = ops.Norm(1 + randn(g, d, std=0.1), randn(g, d, std=0.1)), ops.Norm(1 + randn(g, d, std=0.1), kind="rms"), randn(g, d, std=0.3)
+    per_sample = randn(g, b, d, std=0.5)
+    for gate in (None, per_sample, randn(g, b, n, d, std=0.5)):
+        want, norm = residual_ref(residual, y, pre, post, scale, per_sample[:, None] if gate is per_sample else gate, 1.0)
+        r, x = ops.residual_norm(residual, y, pre_norm=pre, post_norm=post, scale=scale, gate=gate)
+        close(r, *want, "r")
+        close(x, *finish(*norm, torch.bfloat16), "x")
+    h = residual.clone()
+    again = ops.residual_norm(h, y, pre_norm=pre, post_norm=post, scale=scale, gate=gate, out=(h, None))
+    assert again[0] is h and torch.equal(h, r) and torch.equal(again[1], x)
+
+
 def test_residual_norm_keeps_a_large_mean(ops):
     """A row whose mean is 4000 times its spread: a sum of squares minus a squared mean would have nothing left."""
     g = gen(33)
