@@ -130,41 +130,84 @@ template <typename T, int D, bool KEYS> struct Form {
     static_assert(!KEYS || MAPS == 2, "one map per wave: rows only");
 };
 
-// Units of work: a block of query rows of a key head.  The first `full` of them run whole, the rest are split over `splits` workgroups each.
+// Units of work: a block of query rows of a key head.  The first `full` of them run whole, the rest in pieces: `splits` each, or as many as its sequence's
+// length earns it (`shared`).  A piece is a workgroup; those of one split lie beside each other, row blocks innermost: they read the same keys.
 struct Args {
     rz_diff_attention_args a;
     int group, rows, row_blocks;                               // heads per key head, query rows per key head, their blocks
     int units, full, splits;
+    bool shared;
+    int least;                                                 // keys of a piece at least
     float c;                                                   // scale * log2(e)
     int part_rows;                                             // rows of a unit in the workspace
     float* ws;
 };
-// workspace, floats: [unit - full][split][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
+// workspace, floats: [piece][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
 __host__ __device__ inline int64_t parts(const Args& x) { return (int64_t)(x.units - x.full) * x.splits * x.part_rows; }
+constexpr int kMostSplits = 64;                                // the join reads a row's splits by one wave
 
 // a value that is the same in all lanes, into a scalar register (divisions run on the vector unit)
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-struct Work {
-    int unit, split, rb, hk, b;
-    bool whole;
-    __device__ __forceinline__ void place(const Args& x) {
-        rb = x.row_blocks - 1 - scalar(unit % x.row_blocks);   // row blocks innermost: they read the same keys; causal: the longest first
-        const int bh = scalar(unit / x.row_blocks);
-        hk = scalar(bh % x.a.kv_heads);
-        b = scalar(bh / x.a.kv_heads);
-    }
-    __device__ __forceinline__ Work(const Args& x) {
-        const int id = blockIdx.x;
-        whole = id < x.full;
-        if (whole) unit = xcd_remap(id, x.full), split = 0;
-        else {
-            const int t = xcd_remap(id - x.full, gridDim.x - x.full);
-            unit = x.full + scalar(t / x.splits);
-            split = scalar(t % x.splits);
-            whole = x.splits == 1;
+// The lengths of a batch of at most 64 share its batch * splits pieces per unit: lane b holds sequence b's.  1 + [its length / (the sum of all / (pieces - batch))]
+// never add up to more, and no piece is longer than that share.  4 lengths of 7427 .. 11882: 85 -> 82 us; 8 of 18432 .. 32768, one query each: 97 -> 92 us.
+struct Lengths {
+    int n, splits, first;                                      // keys, pieces of each unit, the first piece
+    __device__ __forceinline__ Lengths(const Args& x, int lane) {
+        n = lane < x.a.batch ? min(max(x.a.kv_lens_dev[lane], 0), x.a.n_k) : 0;
+        const uint32_t t = (uint32_t)(n + 63) >> 6;
+        uint32_t sum = t;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        const uint32_t most = (uint32_t)x.a.batch * (uint32_t)(x.splits - 1), share = max((sum + most - 1) / most, 1u);
+        splits = lane < x.a.batch ? min(1 + (int)(t / share), min(max(n / x.least, 1), kMostSplits)) : 0;
+        int end = splits * x.a.kv_heads * x.row_blocks;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(end, o, 64);
+            if (lane >= o) end += below;
         }
-        place(x);
+        first = end - splits * x.a.kv_heads * x.row_blocks;
+    }
+};
+
+struct Work {
+    int rb, hk, b, n;                                          // row block, key head, sequence, its keys
+    int piece, split, splits;
+    bool any;
+    __device__ __forceinline__ Work(const Args& x, int lane) {
+        const int id = blockIdx.x, per_batch = x.a.kv_heads * x.row_blocks;
+        int unit;                                              // of the sequence
+        any = true, piece = split = 0, splits = 1;
+        if (x.shared) {
+            const Lengths all(x, lane);
+            const int total = __builtin_amdgcn_readlane(all.first, 63);              // lanes behind the batch have no pieces
+            const int end = __builtin_amdgcn_readlane(all.splits, 63) * per_batch + total;
+            any = id < end;
+            if (!any) return;
+            piece = xcd_remap(id, end);
+            b = __popcll(__ballot(all.first <= piece && all.splits > 0)) - 1;        // first ascends, every sequence has a piece
+            n = __builtin_amdgcn_readlane(all.n, b);
+            splits = __builtin_amdgcn_readlane(all.splits, b);
+            const int local = piece - __builtin_amdgcn_readlane(all.first, b);
+            split = scalar(local / per_batch);
+            unit = local - split * per_batch;
+        } else {
+            int u;
+            if (id < x.full) u = xcd_remap(id, x.full);
+            else {
+                const int tail = x.units - x.full;
+                piece = xcd_remap(id - x.full, gridDim.x - x.full);
+                split = scalar(piece / tail);
+                u = x.full + piece - split * tail;
+                splits = x.splits;
+            }
+            b = scalar(u / per_batch);
+            unit = u - b * per_batch;
+            n = x.a.kv_lens_dev ? min(max(scalar(x.a.kv_lens_dev[b]), 0), x.a.n_k) : x.a.n_k;
+        }
+        hk = scalar(unit / x.row_blocks);
+        rb = x.row_blocks - 1 - (unit - hk * x.row_blocks);    // causal: the longest first
     }
 };
 
@@ -470,13 +513,13 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     constexpr int W = F::W, BN = F::BN, TILE = F::TILE, BUF = F::BUF, NC = F::NC, MAPS = F::MAPS;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const rz_diff_attention_args& a = x.a;
-    const Work at(x);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Work at(x, lane);
+    if (!at.any) return;
     const int map = MAPS == 1 ? wave & 1 : 0, group = KEYS ? 0 : MAPS == 1 ? wave >> 1 : wave;      // the wave's (first) map, its 32 rows of the unit
     const int row0 = at.rb * F::BR + 32 * group;
 
-    int n = a.n_k;
-    if (a.kv_lens_dev) n = min(max(scalar(a.kv_lens_dev[at.b]), 0), n);
+    const int n = at.n;
     const int shift = a.causal == RZ_CAUSAL_END ? n - a.n_q : 0;
     auto limit = [&](int query) -> int { return a.causal ? min(n, query + 1 + shift) : n; };       // keys that a query may see at most (may be negative)
     int lim;
@@ -485,8 +528,8 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     const int wave_first = limit(scalar(min(row0, x.rows - 1) / x.group));         // keys that every query of the wave sees, but for hidden ones
     const int unit_first = limit(scalar(at.rb * F::BR / x.group));                 // the same of the workgroup
     int begin = 0, stop = end;
-    if (!at.whole) {
-        const int per = scalar(((end + x.splits - 1) / x.splits + 63) / 64 * 64);
+    if (at.splits > 1) {
+        const int per = scalar(((end + at.splits - 1) / at.splits + 63) / 64 * 64);
         begin = min(at.split * per, end);
         stop = min(begin + per, end);
     }
@@ -558,34 +601,40 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     find();
     if (bits_next) fill(mine, j_first + k_next * STEP, bits_next);
     int turn = 0;
-    while (bits_next) {
-        const int j = j_first + k_next * STEP;
-        const uint64_t bits = bits_next;
-        // everything asked for so far has landed; the other buffer's readers are done
-        landed();
-        if constexpr (!KEYS) __syncthreads();
-        ++k_next;
-        find();
-        char* buf = mine + turn * BUF;
-        if (bits_next) fill(mine + (turn ^ 1) * BUF, j_first + k_next * STEP, bits_next);
-        const bool all = bits == below(BN) && j + BN <= wave_first;
-        uint64_t odd = 0;
-        if (a.causal && j + BN > unit_first) {                            // the same for all waves that share the tile
-            odd = odd_keys<T, D, BN>(buf + TILE, lane);
-            if (odd) {
-                if constexpr (!KEYS) __syncthreads();
-                take_odd<T, D, BN>(buf + TILE, lane);
-                if constexpr (KEYS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                else __syncthreads();
+    // a wave behind the last row only copies its share of the tiles
+    auto run = [&](auto live) {
+        while (bits_next) {
+            const int j = j_first + k_next * STEP;
+            const uint64_t bits = bits_next;
+            // everything asked for so far has landed; the other buffer's readers are done
+            landed();
+            if constexpr (!KEYS) __syncthreads();
+            ++k_next;
+            find();
+            char* buf = mine + turn * BUF;
+            if (bits_next) fill(mine + (turn ^ 1) * BUF, j_first + k_next * STEP, bits_next);
+            const bool all = bits == below(BN) && j + BN <= wave_first;
+            uint64_t odd = 0;
+            if (a.causal && j + BN > unit_first) {                            // the same for all waves that share the tile
+                odd = odd_keys<T, D, BN>(buf + TILE, lane);
+                if (odd) {
+                    if constexpr (!KEYS) __syncthreads();
+                    take_odd<T, D, BN>(buf + TILE, lane);
+                    if constexpr (KEYS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    else __syncthreads();
+                }
             }
-        }
-        const uint32_t kt = lds_address(buf) + k_at, vt = lds_address(buf) + v_at;
+            if constexpr (live) {
+                const uint32_t kt = lds_address(buf) + k_at, vt = lds_address(buf) + v_at;
 #pragma unroll
-        for (int kb = 0; kb < BN / 32; ++kb) {
-            wv.block(kt + kb * 32 * S::RB, vt + kb * 32 * S::RB, (uint32_t)(bits >> (32 * kb)), lim - j - 32 * kb, all, (uint32_t)(odd >> (32 * kb)));
+                for (int kb = 0; kb < BN / 32; ++kb)
+                    wv.block(kt + kb * 32 * S::RB, vt + kb * 32 * S::RB, (uint32_t)(bits >> (32 * kb)), lim - j - 32 * kb, all, (uint32_t)(odd >> (32 * kb)));
+            }
+            turn ^= 1;
         }
-        turn ^= 1;
-    }
+    };
+    if (KEYS || row0 < x.rows) run(std::true_type{});
+    else run(std::false_type{});
 
     // ---- the rows' results ----
     const int again = fresh(lane), h = again >> 5, row = row0 + (again & 31), rr = min(row, x.rows - 1), i = rr / x.group, head = at.hk * x.group + rr % x.group;
@@ -642,8 +691,8 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
             for (int k = 0; k < OWN; ++k) o[y][k] = wv.o[y][k];
     }
 
-    if (!at.whole) {
-        const int64_t slot = ((int64_t)(at.unit - x.full) * x.splits + at.split) * x.part_rows + (row - at.rb * F::BR);
+    if (at.splits > 1) {
+        const int64_t slot = (int64_t)at.piece * x.part_rows + (row - at.rb * F::BR);
         float* part = x.ws + slot * 4 * D;
         float* stat = x.ws + parts(x) * 4 * D + slot * 4;
         if (live) {
@@ -723,22 +772,30 @@ template <typename T, int D> __global__ __launch_bounds__(256) void diff_attenti
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int64_t tail = id / x.part_rows;
     if (tail >= x.units - x.full) return;
-    const int unit = x.full + (int)tail, r = (int)(id - tail * x.part_rows), bh = unit / x.row_blocks;
+    const int per_batch = a.kv_heads * x.row_blocks, u = x.full + (int)tail, r = (int)(id - tail * x.part_rows), b = u / per_batch, unit = u - b * per_batch;
     const int row = (x.row_blocks - 1 - unit % x.row_blocks) * block_rows + r;
     if (row >= x.rows) return;
-    const int b = bh / a.kv_heads, i = row / x.group, head = (bh % a.kv_heads) * x.group + row % x.group;
-    const int64_t slot = tail * x.splits * x.part_rows + r;
+    const int i = row / x.group, head = unit / x.row_blocks * x.group + row % x.group;
+    int piece = (int)tail, step = x.units - x.full, splits = x.splits;
+    if (x.shared) {
+        const Lengths all(x, lane);
+        splits = __shfl(all.splits, b, 64);
+        if (splits == 1) return;
+        piece = __shfl(all.first, b, 64) + unit;
+        step = per_batch;
+    }
+    const int64_t slot = (int64_t)piece * x.part_rows + r, next = (int64_t)step * x.part_rows;
     const float* part = x.ws + slot * 4 * D + lane * N;
     const float* stat = x.ws + parts(x) * 4 * D + slot * 4;
     f32x4 st = {-INFINITY, -INFINITY, 0.f, 0.f};
-    if (lane < x.splits) st = *reinterpret_cast<const f32x4*>(stat + (int64_t)lane * x.part_rows * 4);      // at most 64 splits
+    if (lane < splits) st = *reinterpret_cast<const f32x4*>(stat + lane * next * 4);
     const float m0 = wave_max(st[0]), m1 = wave_max(st[1]);
     const float f0 = st[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[0] - m0), f1 = st[1] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[1] - m1);
     const float l0 = wave_sum(st[2] * f0), l1 = wave_sum(st[3] * f1);
     float o[2][N] = {};
-    for (int s = 0; s < x.splits; ++s) {
+    for (int s = 0; s < splits; ++s) {
         const float w0 = __shfl(f0, s, 64), w1 = __shfl(f1, s, 64);
-        const float* p = part + (int64_t)s * x.part_rows * 4 * D;
+        const float* p = part + s * next * 4 * D;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             o[0][e] = fmaf(p[e], w0, o[0][e]);
@@ -772,7 +829,7 @@ int cu_count() {
 template <int D> bool keys_form(int rows) { return D <= 64 && rows <= 32; }
 
 // The units fill the chip's places round by round; what is left for a last round that would leave most of it idle is split over the keys, so that its
-// splits fill one round: at most 64 of them (the join reads them by one wave), each with at least 4 tiles for every wave.
+// pieces fill one round, each with at least 4 tiles for every wave.
 template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& a, void* ws) {
     typedef Form<T, D, KEYS> F;
     Args x;
@@ -785,9 +842,11 @@ template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& 
     const int places = F::kPerCu * cu_count();
     x.full = x.units / places * places;
     const int tail = x.units - x.full;
+    x.least = KEYS ? 4 * F::W * F::BN : 4 * F::BN;
     x.splits = 1;
-    if (tail && (int64_t)tail * 4 <= (int64_t)places * 3) x.splits = max(1, min(min(places / tail, a.n_k / (KEYS ? 4 * F::W * F::BN : 4 * F::BN)), 64));
+    if (tail && (int64_t)tail * 4 <= (int64_t)places * 3) x.splits = max(1, min(min(places / tail, a.n_k / x.least), kMostSplits));
     if (x.splits == 1) x.full = x.units;
+    x.shared = x.splits > 1 && x.full == 0 && a.kv_lens_dev && a.batch <= 64;
     x.part_rows = min(x.rows, F::BR);
     x.ws = (float*)ws;
     return x;

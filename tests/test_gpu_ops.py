@@ -233,6 +233,19 @@ def test_diff_attention_hidden_keys(ops, dtype, causal, keys, shape):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(9, 1, 6000, 4, 2), (9, 65, 5000, 2, 1), (64, 2, 900, 2, 2), (65, 2, 900, 2, 2), (1, 1, 40000, 1, 1), (2, 1, 300000, 1, 1)], ids=str)
+def test_diff_attention_very_unequal_lengths(ops, dtype, shape):
+    """Lengths that share the pieces of the key axis unequally: one long sequence among short, empty and negative ones, all empty, one sequence alone."""
+    b, n_q, n_k, h, hk = shape
+    q, k, v, lam, w = attention_inputs(sum(shape), *shape, 32, dtype)
+    one_long = torch.tensor([0, 1, n_k, -7, 63, 64, 65, n_k // 2, 5], dtype=torch.int32, device="cuda").repeat(8)[:b].contiguous()
+    for lens in (one_long, one_long.flip(0).contiguous(), torch.full_like(one_long, n_k), torch.zeros_like(one_long)):
+        for causal in (None, "end"):
+            got = ops.diff_attention(q, k, v, lam, lambda_init=0.3, causal=causal, kv_lens=lens, norm_weight=w)
+            close(got, *attention_ref(q, k, v, lam, 0.3, causal=causal, lens=lens, norm=w))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_diff_attention_causal_rows_do_not_read_the_future(ops, dtype):
     """A NaN or infinity in a later token reaches that token's and later rows alone, whichever of k and v holds it."""
     b, n, h = 1, 150, 2
