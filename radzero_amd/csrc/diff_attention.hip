@@ -45,12 +45,34 @@ template <> struct Op<float> {
     }
 };
 
+// x = hi + mid + lo exactly: three bf16 with the sign and 8 bits of x's 24 each, cut off (nothing overflows; a part below 2^-126 is lost, an infinity becomes NaN)
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&c)[3]) {
+    u32x4 w[3];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        uint32_t b[2][3];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float r = x[e + i];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                b[i][k] = __float_as_uint(r);
+                r -= __uint_as_float(b[i][k] & 0xffff0000u);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) w[k][e / 2] = __builtin_amdgcn_perm(b[1][k], b[0][k], 0x07060302u);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) c[k] = __builtin_bit_cast(bf16x8, w[k]);
+}
+
 // 32 keys' weights as the product with the values takes them, and this lane's share of their sum
-template <typename T> struct Weights {
-    typename Op<T>::chunk w[2];
+template <typename T, int PLANES> struct Weights {
+    typename Op<T>::chunk w[1][2];
     __device__ __forceinline__ float set(const f32x16& p) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) w[u] = pack8<T>(p[8 * u], p[8 * u + 1], p[8 * u + 2], p[8 * u + 3], p[8 * u + 4], p[8 * u + 5], p[8 * u + 6], p[8 * u + 7]);
+        for (int u = 0; u < 2; ++u) w[0][u] = pack8<T>(p[8 * u], p[8 * u + 1], p[8 * u + 2], p[8 * u + 3], p[8 * u + 4], p[8 * u + 5], p[8 * u + 6], p[8 * u + 7]);
         // the sum of the rounded weights (they then add up to one), two of them to an instruction
         float t[2] = {0.f, 0.f};
 #pragma unroll
@@ -58,21 +80,40 @@ template <typename T> struct Weights {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 if constexpr (std::is_same<T, bf16_t>::value)
-                    t[u] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{w[u][e], w[u][e + 1]}, bf16x2{(bf16_t)1.f, (bf16_t)1.f}, t[u], false);
+                    t[u] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{w[0][u][e], w[0][u][e + 1]}, bf16x2{(bf16_t)1.f, (bf16_t)1.f}, t[u], false);
                 else
-                    t[u] = __builtin_amdgcn_fdot2(f16x2{w[u][e], w[u][e + 1]}, f16x2{(f16_t)1.f, (f16_t)1.f}, t[u], false);
+                    t[u] = __builtin_amdgcn_fdot2(f16x2{w[0][u][e], w[0][u][e + 1]}, f16x2{(f16_t)1.f, (f16_t)1.f}, t[u], false);
             }
         return t[0] + t[1];
     }
 };
-template <> struct Weights<float> {
+__device__ __forceinline__ float sum16(const f32x16& p) {
+    float t[2] = {p[0], p[1]};
+#pragma unroll
+    for (int e = 2; e < 16; ++e) t[e & 1] += p[e];
+    return t[0] + t[1];
+}
+template <> struct Weights<float, 1> {
     f32x16 w;
     __device__ __forceinline__ float set(const f32x16& p) {
         w = p;
-        float t[2] = {p[0], p[1]};
+        return sum16(p);
+    }
+};
+template <> struct Weights<bf16_t, 3> {
+    bf16x8 w[3][2];
+    __device__ __forceinline__ float set(const f32x16& p) {
 #pragma unroll
-        for (int e = 2; e < 16; ++e) t[e & 1] += p[e];
-        return t[0] + t[1];
+        for (int u = 0; u < 2; ++u) {
+            float x[8];
+            bf16x8 c[3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = p[8 * u + e];
+            split8(x, c);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) w[k][u] = c[k];
+        }
+        return sum16(p);
     }
 };
 
@@ -111,15 +152,19 @@ template <typename T, int D> struct Shape {
 
 // How a workgroup shares the work.  MAPS: maps of a wave.  Two share a fragment of the values; head dim 128 would need 256 registers for both O, so there
 // two waves take a map each.  BN: keys of a tile, 64 where the tile buffers of two workgroups fit the LDS, 32 for long rows.
+// PLANES: fp32 products as 6 of the 9 of three bf16 parts each (what is left out is below 2^-23 |a||b|): 192 cycles of the matrix unit for 16 terms where
+// 32x32x2 takes 512.  The parts are made once per tile, on the way to LDS.  The keys form, bound by HBM, keeps 32x32x2.
 template <typename T, int D, bool KEYS> struct Form {
-    static constexpr int RB = Shape<T, D>::RB;
+    static constexpr int PLANES = sizeof(T) == 4 && !KEYS ? 3 : 1;
+    typedef typename std::conditional<PLANES == 3, bf16_t, T>::type M;         // what the matrix unit takes
+    static constexpr int RB = Shape<M, D>::RB;
     static constexpr int MAPS = D == 128 ? 1 : 2;
     static constexpr int W = KEYS ? (RB <= 256 ? 4 : 2) : 4;   // keys: as many private double buffers of 32 keys as 128 KB hold
     static constexpr int BR = KEYS ? 32 : 32 * W * MAPS / 2;   // query rows
-    static constexpr int BN = KEYS ? 32 : RB <= 256 ? 64 : 32;
-    static constexpr int TILE = BN * RB, BUF = 2 * TILE;       // keys, then values
-    static constexpr int NC = Shape<T, D>::NC;
-    static constexpr int kTiles = 2 * BUF * (KEYS ? W : 1);
+    static constexpr int BN = KEYS || PLANES == 3 ? 32 : RB <= 256 ? 64 : 32;
+    static constexpr int TILE = PLANES * BN * RB, BUF = 2 * TILE;                // keys, then values
+    static constexpr int NC = Shape<M, D>::NC;
+    static constexpr int kTiles = PLANES == 3 ? BUF + 16 : 2 * BUF * (KEYS ? W : 1);
     // what the waves exchange at the end: keys, every wave's O, maxima and sums; one map per wave, the second maps' O
     static constexpr int kJoin = KEYS ? W * (2 * 2 * D * 32 + 64) * 4 : MAPS == 1 ? W / 2 * 2 * D * 32 * 4 : 0;
     static constexpr int kLds = kTiles > kJoin ? kTiles : kJoin;
@@ -227,31 +272,51 @@ __device__ __forceinline__ float head_lambda(const rz_diff_attention_args& a, in
 __device__ __forceinline__ uint64_t below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // ---- one wave's 32 query rows ---------------------------------------------------------------------------------------------------
-template <typename T, int D, int MAPS> struct Wave {
+template <typename T, int D, int MAPS, int PLANES> struct Wave {             // T: what the matrix unit takes
     typedef Shape<T, D> S;
     typedef typename Op<T>::chunk chunk;
+    typedef Weights<T, PLANES> W;
     static constexpr int NT = S::NT, NC = S::NC, RB = S::RB;
+    static constexpr int PLANE = 32 * RB;   // bytes from one part of a tile to the next (PLANES == 3: tiles of 32 keys)
 
-    chunk q[MAPS][NT];
+    chunk q[PLANES][MAPS][NT];
     f32x16 o[MAPS][NC];
     float m[MAPS], l[MAPS];                 // reference maximum of the scores in log2 units (-inf: no key yet), this lane's share of the sum
     float c;                          // scale * log2(e)
     int h;                            // which half of every 8 keys the lane holds
     bool started;                     // every row has a reference maximum (wave-uniform)
 
-    __device__ __forceinline__ void init(const Args& x, const T* qrow) {      // qrow: the first of the wave's maps
+    template <typename Q> __device__ __forceinline__ void init(const Args& x, const Q* qrow) {      // qrow: the first of the wave's maps
         c = x.c;
         started = false;
 #pragma unroll
         for (int y = 0; y < MAPS; ++y) {
             m[y] = -INFINITY, l[y] = 0.f;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) q[y][t] = *reinterpret_cast<const chunk*>((const char*)qrow + (y * NT + t) * 32 + h * 16);
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (PLANES == 3) {
+                    const f32x4* p = reinterpret_cast<const f32x4*>(qrow + (y * NT + t) * 16 + h * 8);
+                    const f32x4 a = p[0], b = p[1];
+                    chunk c[3];
+                    split8({a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}, c);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) q[k][y][t] = c[k];
+                } else q[0][y][t] = *reinterpret_cast<const chunk*>((const char*)qrow + (y * NT + t) * 32 + h * 16);
+            }
 #pragma unroll
             for (int cb = 0; cb < NC; ++cb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[y][cb][e] = 0.f;
         }
+    }
+
+    // c + a b of fp32 operands in parts, the smallest products first
+    static __device__ __forceinline__ f32x16 mma(const chunk (&a)[PLANES], const chunk (&b)[PLANES], f32x16 c) {
+#pragma unroll
+        for (int i = PLANES - 1; i >= 0; --i)
+#pragma unroll
+            for (int k = i; k >= 0; --k) c = Op<T>::mma(a[k], b[i - k], c);
+        return c;
     }
 
     // S^T of the 32 keys at kt (k_lane() of their LDS image): register e is key 8 (e / 4) + 4 h + e % 4 of them
@@ -262,7 +327,12 @@ template <typename T, int D, int MAPS> struct Wave {
     __device__ __forceinline__ f32x16 scores(uint32_t kt, int y) const {
         f32x16 s = {};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s = Op<T>::mma(lds_read<chunk>(kt ^ ((y * NT + t) << 5)), q[y][t], s);
+        for (int t = 0; t < NT; ++t) {
+            chunk k[PLANES], x[PLANES];
+#pragma unroll
+            for (int i = 0; i < PLANES; ++i) k[i] = lds_read<chunk>((kt ^ ((y * NT + t) << 5)) + i * PLANE), x[i] = q[i][y][t];
+            s = mma(k, x, s);
+        }
         return s;
     }
 
@@ -298,7 +368,7 @@ template <typename T, int D, int MAPS> struct Wave {
     // The weights of 32 keys without a maximum: one that outgrows the reference shows in the sum.  2^15 keeps every weight below the largest f16.  False: some row's did.
     // One run of instructions from the matrix products to what reads them: with a branch between, the fp32 kernels came out without the wait states they need.
     static constexpr float kMost = 32768.f;
-    template <bool HIDE> __device__ __forceinline__ bool straight(uint32_t kt, uint32_t seen, Weights<T> (&p)[MAPS], float (&t)[MAPS], bool& fine) const {
+    template <bool HIDE> __device__ __forceinline__ bool straight(uint32_t kt, uint32_t seen, W (&p)[MAPS], float (&t)[MAPS], bool& fine) const {
         f32x16 s[MAPS];
 #pragma unroll
         for (int y = 0; y < MAPS; ++y) s[y] = scores(kt, y);
@@ -327,7 +397,7 @@ template <typename T, int D, int MAPS> struct Wave {
             return r0 * RB + (((sub * 2 + ((x & 3) >> 1)) ^ S::swz_v(x >> 2)) << 4) + (x & 1) * 8;
         }
     }
-    __device__ __forceinline__ void values(uint32_t vt, const Weights<T> (&p)[MAPS]) {
+    __device__ __forceinline__ void values(uint32_t vt, const W (&p)[MAPS]) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -343,9 +413,16 @@ template <typename T, int D, int MAPS> struct Wave {
 #pragma unroll
                 for (int cb = 0; cb < NC; ++cb) {
                     const uint32_t at = (vt ^ ((cb & 3) << 6)) + (cb >> 2) * 256 + 16 * u * RB;
-                    const chunk v = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at), tr(at + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
+                    chunk v[PLANES];
 #pragma unroll
-                    for (int y = 0; y < MAPS; ++y) o[y][cb] = Op<T>::mma(v, p[y].w[u], o[y][cb]);
+                    for (int i = 0; i < PLANES; ++i) v[i] = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at + i * PLANE), tr(at + i * PLANE + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int y = 0; y < MAPS; ++y) {
+                        chunk w[PLANES];
+#pragma unroll
+                        for (int i = 0; i < PLANES; ++i) w[i] = p[y].w[i][u];
+                        o[y][cb] = mma(v, w, o[y][cb]);
+                    }
                 }
         }
     }
@@ -353,7 +430,7 @@ template <typename T, int D, int MAPS> struct Wave {
     // 32 keys that stand in LDS at kt, vt.  bits: those that somebody may see; rest: how many of them at most this lane's query sees (its causal end or length);
     // all: every query of the wave sees every key; odd: bit j = key j's values were not all finite (take_odd)
     __device__ __forceinline__ void block(uint32_t kt, uint32_t vt, uint32_t bits, int rest, bool all, uint32_t odd) {
-        Weights<T> p[MAPS];
+        W p[MAPS];
         float t[MAPS];
         auto mine = [&] { return (bits & (uint32_t)below(rest)) >> (4 * h); };
         bool done = false, fine = true;
@@ -442,6 +519,56 @@ template <typename T, int D, int ROWS, int W, bool VALUES> struct Stage {
     }
 };
 
+// The same for fp32 rows in parts: a thread holds its share of the next tile in registers while this one is worked on.
+template <int D, int ROWS, int W> struct Parts {
+    typedef Shape<bf16_t, D> S;
+    static constexpr int N = ROWS * S::CH / (64 * W), per = 64 / S::CH;    // 8 columns of a row each; rows of a wave's instruction
+    const char* src;
+    int64_t stride;
+    f32x4 x[N][2];
+
+    __device__ __forceinline__ void init(const void* p, int64_t bytes) { src = (const char*)p, stride = bytes; }
+    __device__ __forceinline__ void load(int j0, uint32_t bits, int wave, int lane) {
+        const int first = __builtin_ctz(bits);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = (n * W + wave) * per + lane / S::CH, key = j0 + ((bits >> r) & 1 ? r : first);
+            const f32x4* p = reinterpret_cast<const f32x4*>(src + (int64_t)key * stride + lane % S::CH * 32);
+            x[n][0] = p[0], x[n][1] = p[1];
+        }
+    }
+    // Returns, if asked to look for them, the keys (bits) whose values were not all finite; those values are zero then (as by take_odd).
+    template <bool VALUES> __device__ __forceinline__ uint32_t store(char* lds, int wave, int lane, bool look) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = (n * W + wave) * per + lane / S::CH;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = x[n][e / 4][e % 4];
+            if (VALUES && look) {
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const bool finite = fabsf(v[e]) < INFINITY;
+                    bad = bad || !finite;
+                    v[e] = finite ? v[e] : 0.f;
+                }
+                const uint64_t b = __ballot(bad);
+#pragma unroll
+                for (int i = 0; i < per; ++i)
+                    if (b >> (i * S::CH) & ((1ull << S::CH) - 1)) odd |= 1u << ((n * W + wave) * per + i);
+            }
+            bf16x8 c[3];
+            split8(v, c);
+            char* at = lds + r * S::RB + (((lane % S::CH) ^ (VALUES ? S::swz_v(r) : S::swz_k(r))) << 4);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(at + k * ROWS * S::RB) = c[k];
+        }
+        return odd;
+    }
+};
+
 // Values that are not finite, in a tile that not every query sees in full (causal): 0 * inf is not 0, so they would reach queries that must not see them.
 // Returns the keys (bits) that hold any; take_odd then clears those values in LDS, and a query that does see such a key becomes NaN through its sum.
 template <typename T> __device__ __forceinline__ bool odd_chunk(const u32x4& v) {
@@ -509,8 +636,9 @@ __device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, fl
 
 template <typename T, int D, bool KEYS, typename F = Form<T, D, KEYS>>
 __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attention_kernel(const Args x) {
-    typedef Shape<T, D> S;
-    constexpr int W = F::W, BN = F::BN, TILE = F::TILE, BUF = F::BUF, NC = F::NC, MAPS = F::MAPS;
+    typedef Shape<typename F::M, D> S;
+    constexpr int W = F::W, BN = F::BN, TILE = F::TILE, BUF = F::BUF, NC = F::NC, MAPS = F::MAPS, PLANES = F::PLANES;
+    typedef Wave<typename F::M, D, MAPS, PLANES> Rows;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const rz_diff_attention_args& a = x.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -534,7 +662,7 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
         stop = min(begin + per, end);
     }
 
-    Wave<T, D, MAPS> wv;
+    Rows wv;
     wv.h = lane >> 5;
     {
         const int rr = min(row0 + (lane & 31), x.rows - 1), i = rr / x.group, head = at.hk * x.group + rr % x.group;
@@ -542,10 +670,8 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
         wv.init(x, (const T*)a.q_dev + at.b * a.q_batch_stride + i * a.q_token_stride + head * a.q_head_stride + map * D);
     }
 
-    Stage<T, D, BN, KEYS ? 1 : W, false> keys;
-    Stage<T, D, BN, KEYS ? 1 : W, true> values;
-    keys.init((const T*)a.k_dev + at.b * a.k_batch_stride + at.hk * a.k_head_stride, a.k_token_stride * (int64_t)sizeof(T), KEYS ? 0 : wave, lane);
-    values.init((const T*)a.v_dev + at.b * a.v_batch_stride + at.hk * a.v_head_stride, a.v_token_stride * (int64_t)sizeof(T), KEYS ? 0 : wave, lane);
+    const T *k_src = (const T*)a.k_dev + at.b * a.k_batch_stride + at.hk * a.k_head_stride, *v_src = (const T*)a.v_dev + at.b * a.v_batch_stride + at.hk * a.v_head_stride;
+    const int64_t k_step = a.k_token_stride * (int64_t)sizeof(T), v_step = a.v_token_stride * (int64_t)sizeof(T);
     const int64_t* mask = a.mask_dev ? a.mask_dev + at.b * a.mask_batch_stride : nullptr;
     constexpr int STEP = KEYS ? BN * W : BN;
     const int j_first = begin + (KEYS ? wave * BN : 0);
@@ -587,54 +713,97 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
             return;
         }
     };
-    auto fill = [&](char* buf, int j, uint64_t bits) {
-        keys.fill(buf, j, bits, lane);
-        values.fill(buf + TILE, j, bits, lane);
-    };
-    char* mine = lds + (KEYS ? wave * 2 * BUF : 0);
     // the queries are there before the first copy leaves: a wait for them inside the loop would be one for the copies too
 #pragma unroll
-    for (int y = 0; y < MAPS; ++y)
+    for (int k = 0; k < PLANES; ++k)
 #pragma unroll
-        for (int t = 0; t < S::NT; ++t) asm volatile("" : "+v"(wv.q[y][t]));
-    const uint32_t k_at = Wave<T, D, MAPS>::k_lane(lane) + map * (S::RB / 2), v_at = TILE + Wave<T, D, MAPS>::v_lane(lane);
+        for (int y = 0; y < MAPS; ++y)
+#pragma unroll
+            for (int t = 0; t < S::NT; ++t) asm volatile("" : "+v"(wv.q[k][y][t]));
+    const uint32_t k_at = Rows::k_lane(lane) + map * (S::RB / 2), v_at = TILE + Rows::v_lane(lane);
     find();
-    if (bits_next) fill(mine, j_first + k_next * STEP, bits_next);
-    int turn = 0;
     // a wave behind the last row only copies its share of the tiles
-    auto run = [&](auto live) {
-        while (bits_next) {
-            const int j = j_first + k_next * STEP;
-            const uint64_t bits = bits_next;
-            // everything asked for so far has landed; the other buffer's readers are done
-            landed();
-            if constexpr (!KEYS) __syncthreads();
-            ++k_next;
-            find();
-            char* buf = mine + turn * BUF;
-            if (bits_next) fill(mine + (turn ^ 1) * BUF, j_first + k_next * STEP, bits_next);
-            const bool all = bits == below(BN) && j + BN <= wave_first;
-            uint64_t odd = 0;
-            if (a.causal && j + BN > unit_first) {                            // the same for all waves that share the tile
-                odd = odd_keys<T, D, BN>(buf + TILE, lane);
-                if (odd) {
-                    if constexpr (!KEYS) __syncthreads();
-                    take_odd<T, D, BN>(buf + TILE, lane);
-                    if constexpr (KEYS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    else __syncthreads();
-                }
-            }
-            if constexpr (live) {
-                const uint32_t kt = lds_address(buf) + k_at, vt = lds_address(buf) + v_at;
+    const bool idle = !KEYS && row0 >= x.rows;
+    if constexpr (PLANES == 3) {
+        Parts<D, BN, W> keys, values;
+        keys.init(k_src, k_step);
+        values.init(v_src, v_step);
+        uint32_t* odd_keys_of = (uint32_t*)(lds + BUF);                   // of each wave's share of a tile
+        auto load = [&] {
+            const int again = fresh(lane);
+            keys.load(j_first + k_next * STEP, (uint32_t)bits_next, wave, again);
+            values.load(j_first + k_next * STEP, (uint32_t)bits_next, wave, again);
+        };
+        auto run = [&](auto live) {
+            while (bits_next) {
+                const int j = j_first + k_next * STEP, again = fresh(lane);
+                const uint32_t bits = (uint32_t)bits_next;
+                const bool look = a.causal && j + BN > unit_first;        // the same for all waves that share the tile
+                __syncthreads();                                          // the tile before has been read
+                keys.template store<false>(lds, wave, again, false);
+                const uint32_t here = values.template store<true>(lds + TILE, wave, again, look);
+                if (look && lane == 0) odd_keys_of[wave] = here;
+                __syncthreads();
+                ++k_next;
+                find();
+                if (bits_next) load();
+                uint32_t odd = 0;
+                if (look)
 #pragma unroll
-                for (int kb = 0; kb < BN / 32; ++kb)
-                    wv.block(kt + kb * 32 * S::RB, vt + kb * 32 * S::RB, (uint32_t)(bits >> (32 * kb)), lim - j - 32 * kb, all, (uint32_t)(odd >> (32 * kb)));
+                    for (int w = 0; w < W; ++w) odd |= (uint32_t)scalar((int)odd_keys_of[w]);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (live) wv.block(lds_address(lds) + k_at, lds_address(lds) + v_at, bits, lim - j, bits == ~0u && j + BN <= wave_first, odd);
             }
-            turn ^= 1;
-        }
-    };
-    if (KEYS || row0 < x.rows) run(std::true_type{});
-    else run(std::false_type{});
+        };
+        if (bits_next) load();
+        if (!idle) run(std::true_type{});
+        else run(std::false_type{});
+    } else {
+        Stage<T, D, BN, KEYS ? 1 : W, false> keys;
+        Stage<T, D, BN, KEYS ? 1 : W, true> values;
+        keys.init(k_src, k_step, KEYS ? 0 : wave, lane);
+        values.init(v_src, v_step, KEYS ? 0 : wave, lane);
+        auto fill = [&](char* buf, int j, uint64_t bits) {
+            keys.fill(buf, j, bits, lane);
+            values.fill(buf + TILE, j, bits, lane);
+        };
+        char* mine = lds + (KEYS ? wave * 2 * BUF : 0);
+        if (bits_next) fill(mine, j_first + k_next * STEP, bits_next);
+        int turn = 0;
+        auto run = [&](auto live) {
+            while (bits_next) {
+                const int j = j_first + k_next * STEP;
+                const uint64_t bits = bits_next;
+                // everything asked for so far has landed; the other buffer's readers are done
+                landed();
+                if constexpr (!KEYS) __syncthreads();
+                ++k_next;
+                find();
+                char* buf = mine + turn * BUF;
+                if (bits_next) fill(mine + (turn ^ 1) * BUF, j_first + k_next * STEP, bits_next);
+                const bool all = bits == below(BN) && j + BN <= wave_first;
+                uint64_t odd = 0;
+                if (a.causal && j + BN > unit_first) {                    // the same for all waves that share the tile
+                    odd = odd_keys<T, D, BN>(buf + TILE, lane);
+                    if (odd) {
+                        if constexpr (!KEYS) __syncthreads();
+                        take_odd<T, D, BN>(buf + TILE, lane);
+                        if constexpr (KEYS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                        else __syncthreads();
+                    }
+                }
+                if constexpr (live) {
+                    const uint32_t kt = lds_address(buf) + k_at, vt = lds_address(buf) + v_at;
+#pragma unroll
+                    for (int kb = 0; kb < BN / 32; ++kb)
+                        wv.block(kt + kb * 32 * S::RB, vt + kb * 32 * S::RB, (uint32_t)(bits >> (32 * kb)), lim - j - 32 * kb, all, (uint32_t)(odd >> (32 * kb)));
+                }
+                turn ^= 1;
+            }
+        };
+        if (!idle) run(std::true_type{});
+        else run(std::false_type{});
+    }
 
     // ---- the rows' results ----
     const int again = fresh(lane), h = again >> 5, row = row0 + (again & 31), rr = min(row, x.rows - 1), i = rr / x.group, head = at.hk * x.group + rr % x.group;
