@@ -175,21 +175,29 @@ template <typename T, int D, bool KEYS> struct Form {
     static_assert(!KEYS || MAPS == 2, "one map per wave: rows only");
 };
 
-// Units of work: a block of query rows of a key head.  The first `full` of them run whole, the rest in pieces: `splits` each, or as many as its sequence's
-// length earns it (`shared`).  A piece is a workgroup; those of one split lie beside each other, row blocks innermost: they read the same keys.
+// Units of work: a block of query rows of a key head.  The first `full` of them run whole.  The rest, too few for the chip's places, lie end to end as one line of
+// units * blocks blocks of keys, which `ranges` workgroups share evenly: a workgroup's stretch is at most a unit long and ends in one unit or goes on in the next.
+// With lengths (`shared`) each unit is cut into as many pieces as its sequence's length earns it instead; those of one cut lie beside each other, row blocks
+// innermost: they read the same keys.
 struct Args {
     rz_diff_attention_args a;
     int group, rows, row_blocks;                               // heads per key head, query rows per key head, their blocks
-    int units, full, splits;
+    int units, full;
+    int blocks, ranges, each, more;                            // blocks of a unit, of 64 keys (keys form: as many as it has pieces); a workgroup's stretch: `each`, one more for the first `more` of them
     bool shared;
-    int least;                                                 // keys of a piece at least
+    int splits, least;                                         // shared: pieces of a unit on average, keys of a piece at least
     float c;                                                   // scale * log2(e)
-    int part_rows;                                             // rows of a unit in the workspace
+    int part_rows, slots;                                      // rows of a unit in the workspace, its places for pieces
     float* ws;
 };
-// workspace, floats: [piece][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
-__host__ __device__ inline int64_t parts(const Args& x) { return (int64_t)(x.units - x.full) * x.splits * x.part_rows; }
-constexpr int kMostSplits = 64;                                // the join reads a row's splits by one wave
+// workspace, floats: [slot][row] x {O1[2D], O2[2D]}, then m1, m2, l1, l2 of every row
+__host__ __device__ inline int64_t parts(const Args& x) { return (int64_t)x.slots * x.part_rows; }
+constexpr int kMostSplits = 64;                                // the join reads a row's pieces by one wave
+__device__ __forceinline__ int range_begin(const Args& x, int g) { return g * x.each + min(g, x.more); }
+__device__ __forceinline__ int range_of(const Args& x, int block) {
+    const int wide = x.more * (x.each + 1);
+    return block < wide ? block / (x.each + 1) : x.more + (block - wide) / x.each;
+}
 
 // a value that is the same in all lanes, into a scalar register (divisions run on the vector unit)
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -218,41 +226,59 @@ struct Lengths {
 
 struct Work {
     int rb, hk, b, n;                                          // row block, key head, sequence, its keys
-    int piece, split, splits;
+    int lo, hi, of;                                            // the piece: [lo, hi) of `of` equal parts of the keys that the unit sees
+    int slot, range, from, to;                                 // where it goes in the workspace; what is left of the workgroup's stretch
     bool any;
+    __device__ __forceinline__ void unit(const Args& x, int u) {
+        hk = scalar(u / x.row_blocks);
+        rb = x.row_blocks - 1 - (u - hk * x.row_blocks);       // causal: the longest first
+    }
+    __device__ __forceinline__ void place(const Args& x, int u) {
+        const int per_batch = x.a.kv_heads * x.row_blocks;
+        b = scalar(u / per_batch);
+        n = x.a.kv_lens_dev ? min(max(scalar(x.a.kv_lens_dev[b]), 0), x.a.n_k) : x.a.n_k;
+        unit(x, u - b * per_batch);
+    }
+    __device__ __forceinline__ void next(const Args& x) {      // the stretch as far as it lies in one unit
+        const int t = scalar(from / x.blocks);
+        lo = from - t * x.blocks;
+        hi = min(x.blocks, lo + to - from);
+        of = x.blocks;
+        slot = range + t;                                      // ascends by one at least from piece to piece; those of a unit are neighbours
+        from += hi - lo;
+        place(x, x.full + t);
+    }
     __device__ __forceinline__ Work(const Args& x, int lane) {
-        const int id = blockIdx.x, per_batch = x.a.kv_heads * x.row_blocks;
-        int unit;                                              // of the sequence
-        any = true, piece = split = 0, splits = 1;
+        const int id = blockIdx.x;
+        any = true;
+        lo = slot = range = from = to = 0, hi = of = 1;
         if (x.shared) {
+            const int per_batch = x.a.kv_heads * x.row_blocks;
             const Lengths all(x, lane);
-            const int total = __builtin_amdgcn_readlane(all.first, 63);              // lanes behind the batch have no pieces
-            const int end = __builtin_amdgcn_readlane(all.splits, 63) * per_batch + total;
+            const int end = __builtin_amdgcn_readlane(all.first, 63) + __builtin_amdgcn_readlane(all.splits, 63) * per_batch;      // lanes behind the batch: no pieces
             any = id < end;
             if (!any) return;
-            piece = xcd_remap(id, end);
-            b = __popcll(__ballot(all.first <= piece && all.splits > 0)) - 1;        // first ascends, every sequence has a piece
+            slot = xcd_remap(id, end);
+            b = __popcll(__ballot(all.first <= slot && all.splits > 0)) - 1;         // first ascends, every sequence has a piece
             n = __builtin_amdgcn_readlane(all.n, b);
-            splits = __builtin_amdgcn_readlane(all.splits, b);
-            const int local = piece - __builtin_amdgcn_readlane(all.first, b);
-            split = scalar(local / per_batch);
-            unit = local - split * per_batch;
+            of = __builtin_amdgcn_readlane(all.splits, b);
+            const int local = slot - __builtin_amdgcn_readlane(all.first, b);
+            lo = scalar(local / per_batch);
+            hi = lo + 1;
+            unit(x, local - lo * per_batch);
+        } else if (id < x.full) {
+            place(x, xcd_remap(id, x.full));
         } else {
-            int u;
-            if (id < x.full) u = xcd_remap(id, x.full);
-            else {
-                const int tail = x.units - x.full;
-                piece = xcd_remap(id - x.full, gridDim.x - x.full);
-                split = scalar(piece / tail);
-                u = x.full + piece - split * tail;
-                splits = x.splits;
-            }
-            b = scalar(u / per_batch);
-            unit = u - b * per_batch;
-            n = x.a.kv_lens_dev ? min(max(scalar(x.a.kv_lens_dev[b]), 0), x.a.n_k) : x.a.n_k;
+            range = xcd_remap(id - x.full, x.ranges);
+            from = range_begin(x, range);
+            to = range_begin(x, range + 1);
+            next(x);
         }
-        hk = scalar(unit / x.row_blocks);
-        rb = x.row_blocks - 1 - (unit - hk * x.row_blocks);    // causal: the longest first
+    }
+    // the first key of part p: whole blocks of 64
+    __device__ __forceinline__ int key(int p, int end) const {
+        const int blocks = (end + 63) >> 6;
+        return min(end, 64 * (blocks == of ? p : scalar((int)((double)blocks * p / of))));
     }
 };
 
@@ -642,8 +668,9 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const rz_diff_attention_args& a = x.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Work at(x, lane);
+    Work at(x, lane);
     if (!at.any) return;
+    for (;;) {
     const int map = MAPS == 1 ? wave & 1 : 0, group = KEYS ? 0 : MAPS == 1 ? wave >> 1 : wave;      // the wave's (first) map, its 32 rows of the unit
     const int row0 = at.rb * F::BR + 32 * group;
 
@@ -655,12 +682,8 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
     const int end = max(limit(scalar(last / x.group)), 0);                         // of the workgroup
     const int wave_first = limit(scalar(min(row0, x.rows - 1) / x.group));         // keys that every query of the wave sees, but for hidden ones
     const int unit_first = limit(scalar(at.rb * F::BR / x.group));                 // the same of the workgroup
-    int begin = 0, stop = end;
-    if (at.splits > 1) {
-        const int per = scalar(((end + at.splits - 1) / at.splits + 63) / 64 * 64);
-        begin = min(at.split * per, end);
-        stop = min(begin + per, end);
-    }
+    const bool whole = at.lo == 0 && at.hi == at.of;
+    const int begin = whole ? 0 : at.key(at.lo, end), stop = whole ? end : at.key(at.hi, end);
 
     Rows wv;
     wv.h = lane >> 5;
@@ -860,8 +883,8 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
             for (int k = 0; k < OWN; ++k) o[y][k] = wv.o[y][k];
     }
 
-    if (at.splits > 1) {
-        const int64_t slot = (int64_t)at.piece * x.part_rows + (row - at.rb * F::BR);
+    if (!whole) {
+        const int64_t slot = (int64_t)at.slot * x.part_rows + (row - at.rb * F::BR);
         float* part = x.ws + slot * 4 * D;
         float* stat = x.ws + parts(x) * 4 * D + slot * 4;
         if (live) {
@@ -880,7 +903,10 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
                 for (int y = 0; y < MAPS; ++y) stat[map + y] = m[y], stat[2 + map + y] = l[y];
             }
         }
-        return;
+        if (KEYS || at.from == at.to) return;
+        at.next(x);
+        __syncthreads();                                                   // LDS is free for the next piece
+        continue;
     }
     float lambda = 0.f;
     if (a.lambda_head_stride == 0) lambda = head_lambda(a, 0, lane);
@@ -931,6 +957,8 @@ __global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attent
         for (int w = 0; w < W; ++w) ss += stat[w * 32 + (lane & 31)];
     }
     Out<T, D>::template store<OSTEP, OWN>(x, o[0], own0, at.b, i, head, live, norm_factor(a, ss), h);
+    return;                                                                // a whole unit is a workgroup's only piece
+    }
 }
 
 // joins the splits of a query row and head: one wave, a lane owns 4 D / 128 neighbouring columns of both maps
@@ -945,15 +973,19 @@ template <typename T, int D> __global__ __launch_bounds__(256) void diff_attenti
     const int row = (x.row_blocks - 1 - unit % x.row_blocks) * block_rows + r;
     if (row >= x.rows) return;
     const int i = row / x.group, head = unit / x.row_blocks * x.group + row % x.group;
-    int piece = (int)tail, step = x.units - x.full, splits = x.splits;
+    int first, step = 1, splits;
     if (x.shared) {
         const Lengths all(x, lane);
         splits = __shfl(all.splits, b, 64);
-        if (splits == 1) return;
-        piece = __shfl(all.first, b, 64) + unit;
+        first = __shfl(all.first, b, 64) + unit;
         step = per_batch;
+    } else {
+        const int t = (int)tail, g = range_of(x, t * x.blocks);
+        splits = range_of(x, t * x.blocks + x.blocks - 1) - g + 1;
+        first = g + t;
     }
-    const int64_t slot = (int64_t)piece * x.part_rows + r, next = (int64_t)step * x.part_rows;
+    if (splits == 1) return;                                               // it ran whole
+    const int64_t slot = (int64_t)first * x.part_rows + r, next = (int64_t)step * x.part_rows;
     const float* part = x.ws + slot * 4 * D + lane * N;
     const float* stat = x.ws + parts(x) * 4 * D + slot * 4;
     f32x4 st = {-INFINITY, -INFINITY, 0.f, 0.f};
@@ -997,8 +1029,20 @@ int cu_count() {
 // Few rows: the waves of a workgroup share the rows and split the keys (head dims 32 and 64).
 template <int D> bool keys_form(int rows) { return D <= 64 && rows <= 32; }
 
-// The units fill the chip's places round by round; what is left for a last round that would leave most of it idle is split over the keys, so that its
-// pieces fill one round, each with at least 4 tiles for every wave.
+// What the ways to run the last round cost, in microseconds: its longest workgroup, the partial results written and read again (5 TB/s), the join's launch.  A block of
+// 64 keys takes a workgroup `alone` on its CU, or beside one or two others, as long as measured here with 256 of them on every CU, 1024 and 2048 keys.
+template <typename T, int D> struct Cost {
+    static constexpr double alone = sizeof(T) == 4 ? (D == 32 ? 5.0 : D == 64 ? 8.2 : 10.1) : D == 32 ? 1.65 : D == 64 ? 2.24 : 3.07;
+    static constexpr double beside = sizeof(T) == 4 ? 0. : D == 32 ? 0.69 : D == 64 ? 0.82 : 0.29;
+    static constexpr double join = 5., second = 3.;            // a stretch over two units starts and ends twice
+    static double run(int blocks, int64_t groups) { return blocks * (alone + beside * (double)((groups - 1) / cu_count())); }
+    static double pieces(int64_t n, int rows) { return n * (rows * (4. * D * sizeof(float)) * 2 / 5e6); }
+};
+
+// The units fill the chip's places round by round.  The rest, if any, runs whole, in equal pieces or in stretches that share all places, whichever costs least.  Head dim 64,
+// 6 heads, us, whole / equal / stretches: bf16 1370 tokens x 1 59 / 45 / 47, x 3 60 / 69 / 78, 2740 x 1 104 / 74 / 81, 2740 x 2 132 / - / 121, 3800 x 1 142 / 119 / 110;
+// fp32 1370 x 1 184 / 87 / 81, x 2 189 / - / 132.
+// Keys form: as many equal pieces as there are places, if they would leave more than a quarter of them idle, of at least 4 tiles for every wave.
 template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& a, void* ws) {
     typedef Form<T, D, KEYS> F;
     Args x;
@@ -1012,12 +1056,37 @@ template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& 
     x.full = x.units / places * places;
     const int tail = x.units - x.full;
     x.least = KEYS ? 4 * F::W * F::BN : 4 * F::BN;
-    x.splits = 1;
-    if (tail && (int64_t)tail * 4 <= (int64_t)places * 3) x.splits = max(1, min(min(places / tail, a.n_k / x.least), kMostSplits));
-    if (x.splits == 1) x.full = x.units;
-    x.shared = x.splits > 1 && x.full == 0 && a.kv_lens_dev && a.batch <= 64;
+    x.splits = 1, x.shared = false;
+    x.blocks = (a.n_k + 63) / 64, x.ranges = x.each = x.more = x.slots = 0;
     x.part_rows = min(x.rows, F::BR);
     x.ws = (float*)ws;
+    int equal = 1, ranges = 0;
+    if (tail) {
+        // a unit has at most 2 + blocks / each pieces
+        const int most = min(min(places / tail, x.blocks), kMostSplits);
+        if constexpr (KEYS) {
+            if ((int64_t)tail * 4 <= (int64_t)places * 3) equal = max(1, min(most, a.n_k / x.least));
+        } else {
+            typedef Cost<T, D> C;
+            double best = C::run(x.blocks, tail);
+            for (int k = 2; k <= most; ++k) {
+                const double cost = C::run((x.blocks + k - 1) / k, (int64_t)tail * k) + C::pieces((int64_t)tail * k, x.part_rows) + C::join;
+                if (cost < best) best = cost, equal = k;
+            }
+            const int64_t line = (int64_t)tail * x.blocks;
+            const int r = (int)min((int64_t)places, line / ((x.blocks + kMostSplits - 3) / (kMostSplits - 2)));
+            if (r > tail && C::run((int)((line + r - 1) / r), r) + C::pieces(r + tail, x.part_rows) + C::join + C::second < best) ranges = r;
+        }
+    }
+    if (x.full == 0 && a.kv_lens_dev && a.batch <= 64) {
+        x.splits = equal, x.shared = equal > 1;
+        x.slots = x.shared ? tail * equal : 0;
+    } else if (equal > 1 || ranges) {
+        if (!ranges) x.blocks = equal, ranges = tail * equal;              // each piece a stretch of its own
+        const int64_t line = (int64_t)tail * x.blocks;
+        x.ranges = ranges, x.each = (int)(line / ranges), x.more = (int)(line % ranges), x.slots = ranges + tail;
+    }
+    if (!x.shared && !x.ranges) x.full = x.units;
     return x;
 }
 
@@ -1028,7 +1097,7 @@ template <typename T, int D, bool KEYS> hipError_t launch(const rz_diff_attentio
     static const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, F::kLds);
     if (e != hipSuccess) return e;
     const int tail = x.units - x.full;
-    hipLaunchKernelGGL(k, dim3((unsigned)(x.full + tail * x.splits)), dim3(64 * F::W), F::kLds, s, x);
+    hipLaunchKernelGGL(k, dim3((unsigned)(x.shared ? x.slots : x.full + x.ranges)), dim3(64 * F::W), F::kLds, s, x);
     if (hipError_t err = hipGetLastError(); err != hipSuccess || !tail) return err;
     hipLaunchKernelGGL((diff_attention_join_kernel<T, D>), dim3((unsigned)(((int64_t)tail * x.part_rows + 3) / 4)), dim3(256), 0, s, x, F::BR);
     return hipGetLastError();
