@@ -988,22 +988,33 @@ template <typename T, int D> __global__ __launch_bounds__(256) void diff_attenti
     const int64_t slot = (int64_t)first * x.part_rows + r, next = (int64_t)step * x.part_rows;
     const float* part = x.ws + slot * 4 * D + lane * N;
     const float* stat = x.ws + parts(x) * 4 * D + slot * 4;
+    const float lambda = head_lambda(a, head, lane);
     f32x4 st = {-INFINITY, -INFINITY, 0.f, 0.f};
     if (lane < splits) st = *reinterpret_cast<const f32x4*>(stat + lane * next * 4);
     const float m0 = wave_max(st[0]), m1 = wave_max(st[1]);
     const float f0 = st[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[0] - m0), f1 = st[1] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[1] - m1);
     const float l0 = wave_sum(st[2] * f0), l1 = wave_sum(st[3] * f1);
     float o[2][N] = {};
-    for (int s = 0; s < splits; ++s) {
-        const float w0 = __shfl(f0, s, 64), w1 = __shfl(f1, s, 64);
-        const float* p = part + s * next * 4 * D;
+    constexpr int kFly = 4;                                                // pieces on their way at a time; those behind the last: the last, of weight 0
+    for (int s = 0; s < splits; s += kFly) {
+        float p[kFly][2][N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            o[0][e] = fmaf(p[e], w0, o[0][e]);
-            o[1][e] = fmaf(p[2 * D + e], w1, o[1][e]);
+        for (int k = 0; k < kFly; ++k)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int e = 0; e < N; ++e) p[k][y][e] = part[min(s + k, splits - 1) * next * 4 * D + y * 2 * D + e];
+#pragma unroll
+        for (int k = 0; k < kFly; ++k) {
+            const bool there = s + k < splits;
+            const float w0 = there ? __shfl(f0, s + k, 64) : 0.f, w1 = there ? __shfl(f1, s + k, 64) : 0.f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                o[0][e] = fmaf(p[k][0][e], w0, o[0][e]);
+                o[1][e] = fmaf(p[k][1][e], w1, o[1][e]);
+            }
         }
     }
-    const float lambda = head_lambda(a, head, lane);
     const float r0 = l0 == 0.f ? 0.f : 1.f / l0, r1 = l1 == 0.f ? 0.f : lambda / l1;
     float ss = 0.f;
 #pragma unroll
