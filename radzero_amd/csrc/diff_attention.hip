@@ -168,8 +168,8 @@ template <typename T, int D, bool KEYS> struct Form {
     // what the waves exchange at the end: keys, every wave's O, maxima and sums; one map per wave, the second maps' O
     static constexpr int kJoin = KEYS ? W * (2 * 2 * D * 32 + 64) * 4 : MAPS == 1 ? W / 2 * 2 * D * 32 * 4 : 0;
     static constexpr int kLds = kTiles > kJoin ? kTiles : kJoin;
-    // workgroups that a CU holds: LDS, and 512 registers of a SIMD lane (two waves of the 16-bit forms, three of their 64-column values, one of fp32)
-    static constexpr int kWaves = sizeof(T) == 4 ? 1 : D == 32 ? 3 : 2;
+    // workgroups that a CU holds: LDS, and 512 registers of a SIMD lane (two waves of the 16-bit forms, one of fp32; one more with 64-column values)
+    static constexpr int kWaves = (sizeof(T) == 4 ? 1 : 2) + (D == 32);
     static constexpr int kPerCu = kWaves * 4 / W < 160 * 1024 / kLds ? kWaves * 4 / W : 160 * 1024 / kLds;
     static_assert(kLds <= 160 * 1024 && kPerCu >= 1, "LDS");
     static_assert(!KEYS || MAPS == 2, "one map per wave: rows only");
@@ -661,7 +661,7 @@ __device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, fl
 }
 
 template <typename T, int D, bool KEYS, typename F = Form<T, D, KEYS>>
-__global__ __launch_bounds__(64 * F::W, sizeof(T) == 2 ? 2 : 1) void diff_attention_kernel(const Args x) {
+__global__ __launch_bounds__(64 * F::W, F::kWaves) void diff_attention_kernel(const Args x) {
     typedef Shape<typename F::M, D> S;
     constexpr int W = F::W, BN = F::BN, TILE = F::TILE, BUF = F::BUF, NC = F::NC, MAPS = F::MAPS, PLANES = F::PLANES;
     typedef Wave<typename F::M, D, MAPS, PLANES> Rows;
@@ -1043,8 +1043,8 @@ template <int D> bool keys_form(int rows) { return D <= 64 && rows <= 32; }
 // What the ways to run the last round cost, in microseconds: its longest workgroup, the partial results written and read again (5 TB/s), the join's launch.  A block of
 // 64 keys takes a workgroup `alone` on its CU, or beside one or two others, as long as measured here with 256 of them on every CU, 1024 and 2048 keys.
 template <typename T, int D> struct Cost {
-    static constexpr double alone = sizeof(T) == 4 ? (D == 32 ? 5.0 : D == 64 ? 8.2 : 10.1) : D == 32 ? 1.65 : D == 64 ? 2.24 : 3.07;
-    static constexpr double beside = sizeof(T) == 4 ? 0. : D == 32 ? 0.69 : D == 64 ? 0.82 : 0.29;
+    static constexpr double alone = sizeof(T) == 4 ? (D == 32 ? 4.75 : D == 64 ? 8.2 : 10.1) : D == 32 ? 1.65 : D == 64 ? 2.24 : 3.07;
+    static constexpr double beside = sizeof(T) == 4 ? (D == 32 ? 3.2 : 0.) : D == 32 ? 0.69 : D == 64 ? 0.82 : 0.29;
     static constexpr double join = 5., second = 3.;            // a stretch over two units starts and ends twice
     static double run(int blocks, int64_t groups) { return blocks * (alone + beside * (double)((groups - 1) / cu_count())); }
     static double pieces(int64_t n, int rows) { return n * (rows * (4. * D * sizeof(float)) * 2 / 5e6); }
