@@ -1719,6 +1719,7 @@ int rz_diff_attention(const rz_diff_attention_args* a, void* workspace, size_t w
         return fail(RZ_ERR_INVALID, "rz_diff_attention: q, k, v, out and their strides must be multiples of 16 bytes");
     const size_t need = diff_attention_workspace_bytes(*a);
     if (need && (!workspace || workspace_bytes < need)) return fail(RZ_ERR_STATE, "rz_diff_attention: workspace too small (rz_diff_attention_workspace)");
+    if (a->out_dev == a->q_dev || (a->n_k && (a->out_dev == a->k_dev || a->out_dev == a->v_dev))) return fail(RZ_ERR_INVALID, "rz_diff_attention: out must not be q, k or v");
     RZ_HIP(launch_diff_attention(*a, workspace, (hipStream_t)stream));
     return 0;
 }

@@ -45,23 +45,18 @@ template <> struct Op<float> {
     }
 };
 
-// x = hi + mid + lo exactly: three bf16 with the sign and 8 bits of x's 24 each, cut off (nothing overflows; a part below 2^-126 is lost, an infinity becomes NaN)
+// x = hi + mid + lo exactly, three bf16 of 8 bits each: hi cut off (nothing overflows), mid rounded (its rest is 8 bits of either sign, below 2^-16 |x|).  A part
+// below 2^-126 is lost; an infinity becomes NaN.
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&c)[3]) {
     u32x4 w[3];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-        uint32_t b[2][3];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float r = x[e + i];
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                b[i][k] = __float_as_uint(r);
-                r -= __uint_as_float(b[i][k] & 0xffff0000u);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k) w[k][e / 2] = __builtin_amdgcn_perm(b[1][k], b[0][k], 0x07060302u);
+        const uint32_t x0 = __float_as_uint(x[e]), x1 = __float_as_uint(x[e + 1]);
+        const float r0 = x[e] - __uint_as_float(x0 & 0xffff0000u), r1 = x[e + 1] - __uint_as_float(x1 & 0xffff0000u);
+        const uint32_t mid = __builtin_bit_cast(uint32_t, bf16x2{(bf16_t)r0, (bf16_t)r1});
+        w[0][e / 2] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+        w[1][e / 2] = mid;
+        w[2][e / 2] = __builtin_amdgcn_perm(__float_as_uint(r1 - __uint_as_float(mid & 0xffff0000u)), __float_as_uint(r0 - __uint_as_float(mid << 16)), 0x07060302u);
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) c[k] = __builtin_bit_cast(bf16x8, w[k]);
@@ -152,7 +147,7 @@ template <typename T, int D> struct Shape {
 
 // How a workgroup shares the work.  MAPS: maps of a wave.  Two share a fragment of the values; head dim 128 would need 256 registers for both O, so there
 // two waves take a map each.  BN: keys of a tile, 64 where the tile buffers of two workgroups fit the LDS, 32 for long rows.
-// PLANES: fp32 products as 6 of the 9 of three bf16 parts each (what is left out is below 2^-23 |a||b|): 192 cycles of the matrix unit for 16 terms where
+// PLANES: fp32 products as 6 of the 9 of three bf16 parts each (what is left out is below 2^-22 |a||b|): 192 cycles of the matrix unit for 16 terms where
 // 32x32x2 takes 512.  The parts are made once per tile, on the way to LDS.  The keys form, bound by HBM, keeps 32x32x2.
 template <typename T, int D, bool KEYS> struct Form {
     static constexpr int PLANES = sizeof(T) == 4 && !KEYS ? 3 : 1;

@@ -75,6 +75,13 @@ def test_diff_attention_workspace_and_nothing_to_do(lib):
             assert lib.rz_diff_attention(ctypes.byref(a), 8, need, None) == 10001
 
 
+@pytest.mark.parametrize("same", ["q_dev", "k_dev", "v_dev"])
+def test_diff_attention_does_not_write_over_its_inputs(lib, same):
+    a = attention_args(**{**dict(q_dev=1 << 12, k_dev=1 << 13, v_dev=1 << 14), same: 16})
+    assert lib.rz_diff_attention(ctypes.byref(a), 16, 1 << 40, None) == 10001
+    assert b"out must not be" in lib.rz_last_error()
+
+
 def norm_args(**kw):
     a = _lib.RzResidualNormArgs(dtype=1, resid_dtype=0, batch=1, rows=3, dim=768, post_kind=0, pre_kind=1, alpha=1.0, post_eps=0.0, pre_eps=1e-6,
                                 y_dev=16, resid_dev=16, resid_out_dev=16, out_dev=16)
