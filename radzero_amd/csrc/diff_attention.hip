@@ -177,7 +177,7 @@ template <typename T, int D, bool KEYS> struct Form {
 struct Args {
     rz_diff_attention_args a;
     int group, rows, row_blocks;                               // heads per key head, query rows per key head, their blocks
-    int units, full;
+    int units, full, cus;
     int blocks, ranges, each, more;                            // blocks of a unit, of 64 keys (keys form: as many as it has pieces); a workgroup's stretch: `each`, one more for the first `more` of them
     bool shared;
     int splits, least;                                         // shared: pieces of a unit on average, keys of a piece at least
@@ -261,6 +261,13 @@ struct Work {
             lo = scalar(local / per_batch);
             hi = lo + 1;
             unit(x, local - lo * per_batch);
+        } else if (id < x.full && x.a.causal && x.full == x.units) {
+            // The longest first, a key head always on the same XCD if their number allows, and every second round over the CUs backwards: a CU that began with a long
+            // unit goes on with a short one.  14 x 512 tokens, 12 heads of 32 over 4: 33.7 -> 28.2 us; 8192 tokens, 16 heads of 64 over 4: 564 -> 423 us.
+            const int round = scalar(id / x.cus), i = id - round * x.cus, heads = x.a.kv_heads * x.a.batch;
+            const int at = (round & 1) && (round + 1) * x.cus <= x.units && x.cus % 8 == 0 ? round * x.cus + x.cus - 8 - (i & ~7) + (i & 7) : id;
+            const int t = scalar(at / heads);
+            place(x, (at - t * heads) * x.row_blocks + t);
         } else if (id < x.full) {
             place(x, xcd_remap(id, x.full));
         } else {
@@ -1059,6 +1066,7 @@ template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& 
     x.row_blocks = (x.rows + F::BR - 1) / F::BR;
     x.units = x.row_blocks * a.kv_heads * a.batch;
     const int places = F::kPerCu * cu_count();
+    x.cus = cu_count();
     x.full = x.units / places * places;
     const int tail = x.units - x.full;
     x.least = KEYS ? 4 * F::W * F::BN : 4 * F::BN;
@@ -1067,7 +1075,7 @@ template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& 
     x.part_rows = min(x.rows, F::BR);
     x.ws = (float*)ws;
     int equal = 1, ranges = 0;
-    if (tail) {
+    if (tail && (KEYS || !a.causal || !x.full)) {                          // causal rows: after a full round short units are left, whose places free up one by one
         // a unit has at most 2 + blocks / each pieces
         const int most = min(min(places / tail, x.blocks), kMostSplits);
         if constexpr (KEYS) {

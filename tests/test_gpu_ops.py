@@ -246,6 +246,17 @@ def test_diff_attention_very_unequal_lengths(ops, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("causal", ["start", "end"])
+def test_diff_attention_causal_over_several_rounds(ops, dtype, causal):
+    """More blocks of query rows than the chip holds at a time, each row written once whatever the order they run in."""
+    b, n, h, hk = 9, 700, 12, 6
+    q, k, v, lam, w = attention_inputs(17, b, n, n, h, hk, 32, dtype)
+    lens = torch.tensor([n, 1, n // 2, 0, n, 650, 33, n, n], dtype=torch.int32, device="cuda")
+    got = ops.diff_attention(q, k, v, lam, lambda_init=0.3, causal=causal, kv_lens=lens, norm_weight=w, out=torch.full_like(q, 9.0))
+    close(got, *attention_ref(q, k, v, lam, 0.3, causal=causal, lens=lens, norm=w))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_diff_attention_causal_rows_do_not_read_the_future(ops, dtype):
     """A NaN or infinity in a later token reaches that token's and later rows alone, whichever of k and v holds it."""
     b, n, h = 1, 150, 2
