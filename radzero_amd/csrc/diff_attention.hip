@@ -15,6 +15,7 @@
 //   rows  4 waves x 32 rows on the same key tiles (double-buffered in LDS, filled by LDS-DMA): many queries
 //   keys  4 waves on the same 32 rows, every wave its own key tiles, joined in LDS: few queries over many keys
 // Either may also split the keys over workgroups; partial (O, m, l) then go through the workspace and a second kernel joins them.
+#include <atomic>
 #include <type_traits>
 
 #include "rz_common.h"
@@ -963,7 +964,226 @@ __global__ __launch_bounds__(64 * F::W, F::kWaves) void diff_attention_kernel(co
     }
 }
 
-// joins the splits of a query row and head: one wave, a lane owns 4 D / 128 neighbouring columns of both maps
+// a query row's result from both maps' O (a lane: 2 D / 64 neighbouring columns) and sums, by one wave
+template <typename T, int D> __device__ __forceinline__ void finish_row(const Args& x, float (&o)[2][2 * D / 64], float l0, float l1, float lambda, int b, int i, int head, int lane) {
+    constexpr int N = 2 * D / 64;
+    const rz_diff_attention_args& a = x.a;
+    const float r0 = l0 == 0.f ? 0.f : 1.f / l0, r1 = l1 == 0.f ? 0.f : lambda / l1;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        o[0][e] = o[0][e] * r0 - o[1][e] * r1;
+        ss = fmaf(o[0][e], o[0][e], ss);
+    }
+    const float f = norm_factor(a, wave_sum(ss));
+    T* out = (T*)a.out_dev + b * a.out_batch_stride + i * a.out_token_stride + head * a.out_head_stride + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = from_f32<T>(o[0][e] * f * (a.norm_weight_dev ? a.norm_weight_dev[lane * N + e] : 1.f));
+}
+
+// Few query rows (R at most) over many keys, bound by HBM: no matrix unit, whose 32 columns would stay empty.  D / 4 lanes take a key, 8 of its columns each: half of
+// them the first map's, half the second's; 256 / D keys of a wave at a time, kFly such steps on their way.  Every place of a key keeps its own maxima, sums and O of all rows;
+// they meet at the end, in the wave, then in LDS.  Weights stay fp32.
+template <typename T, int D, int R> struct Few {
+    static constexpr int W = 4, BR = R, LK = D / 4, H = LK / 2, KEYS = 64 / LK, kFly = R >= 4 ? 2 : 4;
+    static constexpr int BN = KEYS * kFly;                     // keys of a wave's turn
+    static constexpr int kPerCu = R == 1 ? 4 : R == 2 ? 3 : 2;                   // waves of a SIMD, too: registers
+    static constexpr int kJoin = W * R * 4 * D * 4, kLds = kJoin + W * R * 4 * 4;
+};
+template <int CTRL> __device__ __forceinline__ float dpp(float v) { return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xf, 0xf, true)); }
+// the sum over the H lanes of a map (H = 4, 8, 16); the value of the other map's lanes, the same in all of them
+template <int H> __device__ __forceinline__ float map_sum(float v) {
+    v += dpp<0xB1>(v);                                         // lanes 1 apart, 2 apart, then mirrored in 8 and in 16
+    v += dpp<0x4E>(v);
+    if constexpr (H >= 8) v += dpp<0x141>(v);
+    if constexpr (H >= 16) v += dpp<0x140>(v);
+    return v;
+}
+template <int H> __device__ __forceinline__ float other_map(float v) {
+    if constexpr (H == 4) return dpp<0x141>(v);
+    else if constexpr (H == 8) return dpp<0x140>(v);
+    else return __shfl_xor(v, H, 64);
+}
+template <typename T> struct Eight;                            // 8 columns as they lie in memory
+template <> struct Eight<float> {
+    f32x4 v[2];
+    __device__ __forceinline__ void load(const float* p) { v[0] = reinterpret_cast<const f32x4*>(p)[0], v[1] = reinterpret_cast<const f32x4*>(p)[1]; }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = v[e / 4][e % 4];
+    }
+};
+template <typename T> struct Eight {
+    typename Op<T>::chunk v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const typename Op<T>::chunk*>(p); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = to_f32((T)v[e]);
+    }
+};
+
+template <typename T, int D, int R> __global__ __launch_bounds__(256, (Few<T, D, R>::kPerCu)) void diff_attention_few_kernel(const Args x) {
+    typedef Few<T, D, R> F;
+    constexpr int W = F::W, LK = F::LK, H = F::H, FLY = F::kFly, N = 2 * D / 64;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const rz_diff_attention_args& a = x.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Work at(x, lane);
+    if (!at.any) return;
+    const int shift = a.causal == RZ_CAUSAL_END ? at.n - a.n_q : 0;
+    auto limit = [&](int row) -> int { return a.causal ? min(at.n, scalar(row / x.group) + 1 + shift) : at.n; };
+    const int end = max(limit(x.rows - 1), 0), first = limit(0);           // keys of the last row, of all rows
+    const bool whole = at.lo == 0 && at.hi == at.of;
+    const int begin = whole ? 0 : at.key(at.lo, end), stop = whole ? end : at.key(at.hi, end);
+
+    const int col = lane % LK * 8, place = lane / LK;
+    const int64_t* mask = a.mask_dev ? a.mask_dev + at.b * a.mask_batch_stride : nullptr;
+    const T* k_src = (const T*)a.k_dev + at.b * a.k_batch_stride + at.hk * a.k_head_stride + col;
+    const T* v_src = (const T*)a.v_dev + at.b * a.v_batch_stride + at.hk * a.v_head_stride + col;
+    float q[R][8], o[R][2][8], m[R], l[R];
+    int lim[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int rr = min(r, x.rows - 1), i = scalar(rr / x.group), head = at.hk * x.group + rr - i * x.group;
+        Eight<T> e;
+        e.load((const T*)a.q_dev + at.b * a.q_batch_stride + i * a.q_token_stride + head * a.q_head_stride + col);
+        e.get(q[r]);
+        lim[r] = limit(rr);
+        m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[r][0][c] = o[r][1][c] = 0.f;
+    }
+    for (int j0 = begin + wave * F::BN; j0 < stop; j0 += W * F::BN) {
+        Eight<T> kr[FLY], vr[FLY];
+        bool seen[FLY];
+#pragma unroll
+        for (int u = 0; u < FLY; ++u) {
+            const int j = j0 + u * F::KEYS + place, key = min(j, stop - 1);
+            kr[u].load(k_src + key * a.k_token_stride);
+            vr[u].load(v_src + key * a.v_token_stride);
+            seen[u] = j < stop && (!mask || mask[key] != 0);
+        }
+        const bool edge = j0 + F::BN > first;                  // causal: keys that not every row sees
+        float s[R][FLY];
+#pragma unroll
+        for (int u = 0; u < FLY; ++u) {
+            float k[8];
+            kr[u].get(k);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float t = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) t = fmaf(q[r][c], k[c], t);
+                t = map_sum<H>(t) * x.c;
+                s[r][u] = seen[u] && (!edge || j0 + u * F::KEYS + place < lim[r]) ? t : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float top = s[r][0];
+#pragma unroll
+            for (int u = 1; u < FLY; ++u) top = fmaxf(top, s[r][u]);
+            if (__any(top > m[r])) {
+                const float mn = fmaxf(m[r], top), f0 = m[r] == mn ? 1.f : __builtin_amdgcn_exp2f(m[r] - mn), f1 = other_map<H>(f0);
+                const float own = lane % LK < H ? f0 : f1, other = lane % LK < H ? f1 : f0;
+                m[r] = mn;
+                l[r] *= f0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[r][0][c] *= own, o[r][1][c] *= other;
+            }
+            const float ref = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+            for (int u = 0; u < FLY; ++u) {
+                s[r][u] = __builtin_amdgcn_exp2f(s[r][u] - ref);
+                l[r] += s[r][u];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < FLY; ++u) {
+            float v[8];
+            vr[u].get(v);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = seen[u] ? v[c] : 0.f;       // 0 * (what a hidden place holds) would not be 0
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float mine = s[r][u], theirs = other_map<H>(mine);
+                const float p0 = lane % LK < H ? mine : theirs, p1 = lane % LK < H ? theirs : mine;
+                if (edge) {
+                    const bool sees = j0 + u * F::KEYS + place < lim[r];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const float w = sees ? v[c] : 0.f;
+                        o[r][0][c] = fmaf(p0, w, o[r][0][c]);
+                        o[r][1][c] = fmaf(p1, w, o[r][1][c]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        o[r][0][c] = fmaf(p0, v[c], o[r][0][c]);
+                        o[r][1][c] = fmaf(p1, v[c], o[r][1][c]);
+                    }
+                }
+            }
+        }
+    }
+
+    // the places of a wave, then the waves: O [wave][row][map][2 D], {m1, m2, l1, l2} [wave][row]
+    float* f = (float*)lds;
+    f32x4* stat = (f32x4*)(lds + F::kJoin);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float mx = m[r];
+#pragma unroll
+        for (int d = LK; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+        const float g = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - mx), h = other_map<H>(g), g0 = lane % LK < H ? g : h, g1 = lane % LK < H ? h : g;
+        float sum = l[r] * g;
+#pragma unroll
+        for (int d = LK; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+        const float mo = other_map<H>(mx), so = other_map<H>(sum);
+        if (lane == 0) stat[wave * R + r] = f32x4{mx, mo, sum, so};
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                float t = o[r][y][c] * (y ? g1 : g0);
+#pragma unroll
+                for (int d = LK; d < 64; d <<= 1) t += __shfl_xor(t, d, 64);
+                if (place == 0) f[((wave * R + r) * 2 + y) * 2 * D + col + c] = t;
+            }
+    }
+    __syncthreads();
+    for (int r = wave; r < x.rows; r += W) {
+        f32x4 st[W];
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, t[2][N] = {};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            st[w] = stat[w * R + r];
+            m0 = fmaxf(m0, st[w][0]), m1 = fmaxf(m1, st[w][1]);
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float g0 = st[w][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[w][0] - m0), g1 = st[w][1] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[w][1] - m1);
+            l0 = fmaf(st[w][2], g0, l0), l1 = fmaf(st[w][3], g1, l1);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                t[0][e] = fmaf(f[((w * R + r) * 2 + 0) * 2 * D + lane * N + e], g0, t[0][e]);
+                t[1][e] = fmaf(f[((w * R + r) * 2 + 1) * 2 * D + lane * N + e], g1, t[1][e]);
+            }
+        }
+        if (whole) {
+            const int i = scalar(r / x.group), head = at.hk * x.group + r - i * x.group;
+            finish_row<T, D>(x, t, l0, l1, head_lambda(a, a.lambda_head_stride ? head : 0, lane), at.b, i, head, lane);
+        } else {
+            const int64_t slot = (int64_t)at.slot * x.part_rows + r;
+            float* part = x.ws + slot * 4 * D + lane * N;
+#pragma unroll
+            for (int e = 0; e < N; ++e) part[e] = t[0][e], part[2 * D + e] = t[1][e];
+            if (lane == 0) *reinterpret_cast<f32x4*>(x.ws + parts(x) * 4 * D + slot * 4) = f32x4{m0, m1, l0, l1};
+        }
+    }
+}
+
+// joins the pieces of a query row and head: one wave, a lane owns 2 D / 64 neighbouring columns of both maps
 template <typename T, int D> __global__ __launch_bounds__(256) void diff_attention_join_kernel(const Args x, int block_rows) {
     constexpr int N = 2 * D / 64;
     const rz_diff_attention_args& a = x.a;
@@ -1017,17 +1237,7 @@ template <typename T, int D> __global__ __launch_bounds__(256) void diff_attenti
             }
         }
     }
-    const float r0 = l0 == 0.f ? 0.f : 1.f / l0, r1 = l1 == 0.f ? 0.f : lambda / l1;
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        o[0][e] = o[0][e] * r0 - o[1][e] * r1;
-        ss = fmaf(o[0][e], o[0][e], ss);
-    }
-    const float f = norm_factor(a, wave_sum(ss));
-    T* out = (T*)a.out_dev + b * a.out_batch_stride + i * a.out_token_stride + head * a.out_head_stride + lane * N;
-#pragma unroll
-    for (int e = 0; e < N; ++e) out[e] = from_f32<T>(o[0][e] * f * (a.norm_weight_dev ? a.norm_weight_dev[lane * N + e] : 1.f));
+    finish_row<T, D>(x, o, l0, l1, lambda, b, i, head, lane);
 }
 
 int cu_count() {
@@ -1039,8 +1249,13 @@ int cu_count() {
     return n;
 }
 
+// Hardly any rows: no matrix unit.  us, with it / without, head dim 64: bf16, one row, 1 x 6 heads over 257 keys 12.8 / 10.4, 64 x 12 over 300 42 / 24; two rows 43 / 26, but
+// 8 x 4 over 300 12.8 / 15.7: only where every CU has a unit; four rows 43 / 56.  fp32, four rows, 8 x 4 over 8192 120 / 55.
+template <typename T> bool few_form(const rz_diff_attention_args& a, int64_t rows) {
+    return rows <= (sizeof(T) == 4 ? 4 : 1) || (rows == 2 && (int64_t)a.batch * a.kv_heads >= cu_count());
+}
 // Few rows: the waves of a workgroup share the rows and split the keys (head dims 32 and 64).
-template <int D> bool keys_form(int rows) { return D <= 64 && rows <= 32; }
+template <int D> bool keys_form(int64_t rows) { return D <= 64 && rows <= 32; }
 
 // What the ways to run the last round cost, in microseconds: its longest workgroup, the partial results written and read again (5 TB/s), the join's launch.  A block of
 // 64 keys takes a workgroup `alone` on its CU, or beside one or two others, as long as measured here with 256 of them on every CU, 1024 and 2048 keys.
@@ -1056,8 +1271,7 @@ template <typename T, int D> struct Cost {
 // 6 heads, us, whole / equal / stretches: bf16 1370 tokens x 1 59 / 45 / 47, x 3 60 / 69 / 78, 2740 x 1 104 / 74 / 81, 2740 x 2 132 / - / 121, 3800 x 1 142 / 119 / 110;
 // fp32 1370 x 1 184 / 87 / 81, x 2 189 / - / 132.
 // Keys form: as many equal pieces as there are places, if they would leave more than a quarter of them idle, of at least 4 tiles for every wave.
-template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& a, void* ws) {
-    typedef Form<T, D, KEYS> F;
+template <typename T, int D, bool KEYS, typename F> Args make(const rz_diff_attention_args& a, void* ws) {
     Args x;
     x.a = a;
     x.c = a.scale * 1.44269504088896340736f;
@@ -1104,12 +1318,17 @@ template <typename T, int D, bool KEYS> Args make(const rz_diff_attention_args& 
     return x;
 }
 
-template <typename T, int D, bool KEYS> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
-    typedef Form<T, D, KEYS> F;
-    const Args x = make<T, D, KEYS>(a, ws);
-    auto* k = diff_attention_kernel<T, D, KEYS>;
-    static const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, F::kLds);
-    if (e != hipSuccess) return e;
+template <typename T, int D, bool KEYS, typename F> hipError_t launch(void (*k)(Args), const rz_diff_attention_args& a, void* ws, hipStream_t s) {
+    const Args x = make<T, D, KEYS, F>(a, ws);
+    if (F::kLds > 64 * 1024) {
+        static std::atomic<uint64_t> told{0};                              // devices that know
+        int dev = 0;
+        if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+        if (dev >= 64 || !(told.load(std::memory_order_relaxed) >> dev & 1)) {
+            if (hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, F::kLds); e != hipSuccess) return e;
+            if (dev < 64) told.fetch_or(1ull << dev, std::memory_order_relaxed);
+        }
+    }
     const int tail = x.units - x.full;
     hipLaunchKernelGGL(k, dim3((unsigned)(x.shared ? x.slots : x.full + x.ranges)), dim3(64 * F::W), F::kLds, s, x);
     if (hipError_t err = hipGetLastError(); err != hipSuccess || !tail) return err;
@@ -1117,17 +1336,23 @@ template <typename T, int D, bool KEYS> hipError_t launch(const rz_diff_attentio
     return hipGetLastError();
 }
 
+// One of the forms for these sizes: use(KEYS, form, kernel).
+template <typename T, int D, typename Use> auto with_form(const rz_diff_attention_args& a, Use use) {
+    const int64_t rows = (int64_t)a.n_q * (a.heads / a.kv_heads);
+    if (few_form<T>(a, rows)) {
+        if (rows == 1) return use(std::true_type{}, Few<T, D, 1>{}, diff_attention_few_kernel<T, D, 1>);
+        if (rows == 2) return use(std::true_type{}, Few<T, D, 2>{}, diff_attention_few_kernel<T, D, 2>);
+        if constexpr (sizeof(T) == 4) return use(std::true_type{}, Few<T, D, 4>{}, diff_attention_few_kernel<T, D, 4>);
+    }
+    if constexpr (D <= 64)
+        if (keys_form<D>(rows)) return use(std::true_type{}, Form<T, D, true>{}, diff_attention_kernel<T, D, true>);
+    return use(std::false_type{}, Form<T, D, false>{}, diff_attention_kernel<T, D, false>);
+}
 template <typename T, int D> size_t workspace(const rz_diff_attention_args& a) {
-    const int rows = a.n_q * (a.heads / a.kv_heads);
-    Args x;
-    if constexpr (D <= 64) x = keys_form<D>(rows) ? make<T, D, true>(a, nullptr) : make<T, D, false>(a, nullptr);
-    else x = make<T, D, false>(a, nullptr);
-    return (size_t)parts(x) * (4 * D + 4) * sizeof(float);
+    return with_form<T, D>(a, [&](auto keys, auto form, auto) { return (size_t)parts(make<T, D, decltype(keys)::value, decltype(form)>(a, nullptr)) * (4 * D + 4) * sizeof(float); });
 }
 template <typename T, int D> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
-    if constexpr (D <= 64)
-        if (keys_form<D>(a.n_q * (a.heads / a.kv_heads))) return launch<T, D, true>(a, ws, s);
-    return launch<T, D, false>(a, ws, s);
+    return with_form<T, D>(a, [&](auto keys, auto form, auto kernel) { return launch<T, D, decltype(keys)::value, decltype(form)>(kernel, a, ws, s); });
 }
 template <typename T> size_t workspace(const rz_diff_attention_args& a) {
     return a.head_dim == 32 ? workspace<T, 32>(a) : a.head_dim == 64 ? workspace<T, 64>(a) : workspace<T, 128>(a);
