@@ -10,11 +10,15 @@
 // A wave owns 32 query rows (query-major, the heads that share a key head beside each other, so that one tile of keys serves all of them) and computes
 // everything transposed on 32x32 MFMAs: S^T = K Q^T puts a query in a column = in a lane, so that its maximum, its sum and every rescale are
 // that lane's own; P^T then is the B operand of O^T = V^T P^T as it stands in the registers, and one fragment of V^T serves both maps.
-//   16-bit: 32x32x16, V^T fragments by transposing LDS reads;  fp32: 32x32x2 (exact), V^T fragments are plain reads of a row.
-// Two ways to share the work:
-//   rows  4 waves x 32 rows on the same key tiles (double-buffered in LDS, filled by LDS-DMA): many queries
-//   keys  4 waves on the same 32 rows, every wave its own key tiles, joined in LDS: few queries over many keys
-// Either may also split the keys over workgroups; partial (O, m, l) then go through the workspace and a second kernel joins them.
+//   16-bit: 32x32x16, V^T fragments by transposing LDS reads, weights rounded to the type as any such product's operands are;  fp32: the same from three bf16
+//   parts of every operand (rows), or 32x32x2, whose V^T fragments are plain reads of a row (keys).
+// Three ways to share the work:
+//   rows  4 waves x 32 rows on the same key tiles (16-bit: double-buffered in LDS, filled by LDS-DMA): many queries.  Bound by the matrix unit and the
+//         exponentials, whose times add on a SIMD: bf16, 4 x 5330 tokens, 6 heads of 64: 527 us, 994 TFLOP/s executed (12 d per query and key)
+//   keys  4 waves on the same 32 rows, every wave its own key tiles, joined in LDS: few queries over many keys.  Bound by HBM: 16 heads over 4 key heads, 8
+//         caches of 18432 .. 32768 tokens, bf16: 91 us, 4.6 TB/s
+//   few   a handful of rows without the matrix unit: fp32, 8 x 4 key heads x 8192 tokens: 52 us, 5.2 TB/s
+// Each may also split the keys over workgroups; partial (O, m, l) then go through the workspace and a second kernel joins them.
 #include <atomic>
 #include <type_traits>
 

@@ -8,7 +8,7 @@
 // Bound by HBM: every head is read and written once.  The angles of a token are the same in all heads of q and k: a workgroup takes a few
 // tokens, writes their cosines and sines to LDS once and then streams all heads of both tensors past that table.
 // Angles are formed in 64 bits: in fp32 the product of a position near 2^20 and a frequency near 1 is off by 2^-4 radian.  Only the
-// fraction of a turn, in fp32, goes through sin and cos (2e-7 radian).
+// fraction of a turn, in fp32, goes through sin and cos (2e-7 radian).  32 x 5330 tokens, 12 + 12 heads of 64, bf16: 203 us, 5.2 TB/s; one token: the launch, 4 us.
 #include "rz_common.h"
 #include "rz_kernels.h"
 
