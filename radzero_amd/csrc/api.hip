@@ -1701,7 +1701,8 @@ static const char* diff_attention_error(const rz_diff_attention_args* a) {
     if (!(a->scale > 0.f) || a->scale > 1e30f) return "rz_diff_attention: scale must be positive and finite";
     if (a->norm_weight_dev && !(a->norm_eps >= 0.f)) return "rz_diff_attention: norm_eps must not be negative";
     // 32-bit row numbers and grids inside; offsets are 64-bit
-    if (a->n_k > (1 << 30) || (int64_t)a->n_q * a->heads > (1 << 30) || (int64_t)a->batch * a->heads * a->n_q > INT32_MAX)
+    if (a->n_k > (1 << 30) || (int64_t)a->n_q * a->heads > (1 << 30) || (int64_t)a->batch * a->heads * a->n_q > INT32_MAX ||
+        (int64_t)a->batch * a->kv_heads * ((int64_t)a->n_q * (a->heads / a->kv_heads) / 64 + 1) > (1 << 23))         // workgroups: a launch takes less than 2^32 threads
         return "rz_diff_attention: too many rows";
     return nullptr;
 }

@@ -524,16 +524,18 @@ template <typename T, int D, int ROWS, int W, bool VALUES> struct Stage {
     int64_t stride;
     int w;
     uint32_t in;                                                           // a lane's row, from the first of its instruction
+    bool near;                                                             // every such offset fits 32 bits
     static __device__ __forceinline__ int swz(int r) { return VALUES ? S::swz_v(r) : S::swz_k(r); }
 
     __device__ __forceinline__ void init(const void* p, int64_t bytes, int wave, int lane) {
         src = (const char*)p, stride = bytes, w = wave;
         in = (uint32_t)(lane / S::CH) * (uint32_t)stride;
+        near = stride >= 0 && stride < (1 << 28);
     }
     __device__ __forceinline__ void fill(char* lds, int j0, uint64_t bits, int lane) const {
         lane = fresh(lane);
         const int sub = lane / S::CH, cp = lane % S::CH ^ swz(sub);        // a row's XOR is that of its instruction's first row and its own place behind it
-        if (bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1)) {    // every key: a uniform address and a lane's offset
+        if (near && bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1)) {        // every key: a uniform address and a lane's offset
             const char* base = src + (j0 + w * N * per) * stride;
 #pragma unroll
             for (int i = 0; i < N; ++i, base += per * stride) {
@@ -1307,7 +1309,7 @@ template <typename T, int D, bool KEYS, typename F> Args make(const rz_diff_atte
             }
             const int64_t line = (int64_t)tail * x.blocks;
             const int r = (int)min((int64_t)places, line / ((x.blocks + kMostSplits - 3) / (kMostSplits - 2)));
-            if (r > tail && C::run((int)((line + r - 1) / r), r) + C::pieces(r + tail, x.part_rows) + C::join + C::second < best) ranges = r;
+            if (r > tail && line <= INT32_MAX && C::run((int)((line + r - 1) / r), r) + C::pieces(r + tail, x.part_rows) + C::join + C::second < best) ranges = r;
         }
     }
     if (x.full == 0 && a.kv_lens_dev && a.batch <= 64) {

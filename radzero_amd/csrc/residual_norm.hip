@@ -12,6 +12,8 @@
 // 8 x 1370 rows of 1001 (f16): 18.9 us, 4.7 TB/s; a few rows: the launch.  Tried and left: the vectors kept in registers over several rows of
 // a wave, the next row prefetched (418 us: 193 registers, two waves a SIMD), loads past the caches (no change; 25 us at the odd width, where
 // two rows share a line).
+#include <algorithm>
+
 #include "rz_common.h"
 #include "rz_kernels.h"
 
@@ -19,6 +21,7 @@ namespace rz {
 
 namespace {
 
+constexpr int kMostBlocks = 1 << 20;   // workgroups of a launch: a launch takes less than 2^32 threads
 constexpr int kVec = 4;           // columns per chunk: 768 = 3 chunks per lane of a wave, no lane idle
 
 // rows need no alignment beyond their element's: odd widths put every second row off 16 bytes, and the hardware takes such vector accesses
@@ -126,11 +129,11 @@ __device__ __forceinline__ void norm_row(float (&v)[NC][4], int kind, const floa
 }
 
 template <typename T, typename RT, int TPR, int NC, bool STREAM>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(const rz_residual_norm_args a, int total_rows) {
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(const rz_residual_norm_args a, int from_row, int total_rows) {
     __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1, WHOLE = kWhole<TPR, NC>;       // rows per workgroup
     const int lane = threadIdx.x % TPR, dim = a.dim;
-    const int64_t first = (int64_t)blockIdx.x * RPB + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+    const int64_t first = from_row + (int64_t)blockIdx.x * RPB + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
     if (first >= total_rows) return;                      // whole waves, and never a part of a workgroup that shares a row
     const unsigned row = (unsigned)first, batch = row / (unsigned)a.rows;
     const int64_t b = batch, n = row - batch * (unsigned)a.rows;
@@ -178,7 +181,9 @@ template <typename T, typename RT, bool STREAM> hipError_t launch(const rz_resid
 #define RZ_ROWS(TPR, NC)                                                                                                        \
     if (chunks <= TPR * NC) {                                                                                                   \
         constexpr int kBlock = TPR < 256 ? 256 : TPR, kRpb = kBlock / TPR;                                                      \
-        hipLaunchKernelGGL((residual_norm_kernel<T, RT, TPR, NC, STREAM>), dim3((unsigned)((rows - 1) / kRpb + 1)), dim3(kBlock), 0, s, a, rows); \
+        for (int64_t from = 0; from < rows; from += (int64_t)kMostBlocks * kRpb)                                                \
+            hipLaunchKernelGGL((residual_norm_kernel<T, RT, TPR, NC, STREAM>), dim3((unsigned)std::min<int64_t>(kMostBlocks, (rows - from - 1) / kRpb + 1)), \
+                               dim3(kBlock), 0, s, a, (int)from, rows);                                                         \
         return hipGetLastError();                                                                                               \
     }
     RZ_ROWS(64, 1) RZ_ROWS(64, 2) RZ_ROWS(64, 3) RZ_ROWS(64, 4) RZ_ROWS(256, 2) RZ_ROWS(256, 4) RZ_ROWS(256, 8) RZ_ROWS(1024, 4)

@@ -9,6 +9,8 @@
 // tokens, writes their cosines and sines to LDS once and then streams all heads of both tensors past that table.
 // Angles are formed in 64 bits: in fp32 the product of a position near 2^20 and a frequency near 1 is off by 2^-4 radian.  Only the
 // fraction of a turn, in fp32, goes through sin and cos (2e-7 radian).  32 x 5330 tokens, 12 + 12 heads of 64, bf16: 203 us, 5.2 TB/s; one token: the launch, 4 us.
+#include <algorithm>
+
 #include "rz_common.h"
 #include "rz_kernels.h"
 
@@ -87,28 +89,30 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(Heads q, Heads k, cons
                                                           const double* freqs, float amplitude, int64_t total_tokens, int tokens, int head_dim, int P,
                                                           int per_block) {
     __shared__ float2 tab[kTable];
-    const int64_t t0 = (int64_t)blockIdx.x * per_block;
-    const int here = (int)min((int64_t)per_block, total_tokens - t0);
     const int per_axis = P / axes;
-    for (int i = threadIdx.x; i < here * P; i += kThreads) {
-        const int t = i / P, p = i - t * P;
-        const int64_t row = t0 + t, b = row / tokens, n = row - b * tokens;
-        const double angle = (double)positions[b * pos_batch + n * pos_token + p / per_axis] * freqs[p];
-        const double turns = angle * 0.15915494309189533577;                    // 1 / (2 pi)
-        float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        tab[i] = make_float2(amplitude * c, amplitude * s);
-    }
-    __syncthreads();
-    const int tail = head_dim - 2 * P;
-    const int runs = (LAYOUT == RZ_ROTARY_HALF ? P / V : 2 * P / V) + (tail + V - 1) / V;
-    const int heads = q.heads + k.heads, units = heads * runs;
-    for (int i = threadIdx.x; i < here * units; i += kThreads) {
-        const int t = i / units, u = i - t * units, h = u / runs, c = u - h * runs;
-        const int64_t row = t0 + t, b = row / tokens, n = row - b * tokens;
-        const Heads& x = h < q.heads ? q : k;
-        const int hh = h < q.heads ? h : h - q.heads;
-        turn<T, LAYOUT, V, LOOSE>((const T*)x.in + b * x.ib + n * x.it + hh * x.ih, (T*)x.out + b * x.ob + n * x.ot + hh * x.oh, c, P, tail, tab + t * P);
+    for (int64_t t0 = (int64_t)blockIdx.x * per_block; t0 < total_tokens; t0 += (int64_t)gridDim.x * per_block) {
+        const int here = (int)min((int64_t)per_block, total_tokens - t0);
+        for (int i = threadIdx.x; i < here * P; i += kThreads) {
+            const int t = i / P, p = i - t * P;
+            const int64_t row = t0 + t, b = row / tokens, n = row - b * tokens;
+            const double angle = (double)positions[b * pos_batch + n * pos_token + p / per_axis] * freqs[p];
+            const double turns = angle * 0.15915494309189533577;                    // 1 / (2 pi)
+            float s, c;
+            sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+            tab[i] = make_float2(amplitude * c, amplitude * s);
+        }
+        __syncthreads();
+        const int tail = head_dim - 2 * P;
+        const int runs = (LAYOUT == RZ_ROTARY_HALF ? P / V : 2 * P / V) + (tail + V - 1) / V;
+        const int heads = q.heads + k.heads, units = heads * runs;
+        for (int i = threadIdx.x; i < here * units; i += kThreads) {
+            const int t = i / units, u = i - t * units, h = u / runs, c = u - h * runs;
+            const int64_t row = t0 + t, b = row / tokens, n = row - b * tokens;
+            const Heads& x = h < q.heads ? q : k;
+            const int hh = h < q.heads ? h : h - q.heads;
+            turn<T, LAYOUT, V, LOOSE>((const T*)x.in + b * x.ib + n * x.it + hh * x.ih, (T*)x.out + b * x.ob + n * x.ot + hh * x.oh, c, P, tail, tab + t * P);
+        }
+        __syncthreads();                                                            // the table's readers are done
     }
 }
 
@@ -128,7 +132,7 @@ template <typename T, int LAYOUT> hipError_t launch(const rz_rotary_args& a, hip
     // would leave CUs without work
     int per = kTable / P < 8 ? kTable / P : 8;
     while (per > 1 && (total + per - 1) / per < 1024) per /= 2;
-    const dim3 grid((unsigned)((total + per - 1) / per));
+    const dim3 grid((unsigned)std::min<int64_t>((total + per - 1) / per, 1 << 20));       // a launch takes less than 2^32 threads
 #define RZ_TURN(V, LOOSE)                                                                                                                \
     hipLaunchKernelGGL((rotary_kernel<T, LAYOUT, V, LOOSE>), grid, dim3(kThreads), 0, s, q, k, a.positions_dev, a.positions_batch_stride, \
                        a.positions_token_stride, a.n_axes, a.freqs_dev, a.amplitude, total, a.tokens, a.head_dim, P, per)

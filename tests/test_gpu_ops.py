@@ -328,6 +328,34 @@ def test_diff_attention_offsets_beyond_32_bits(ops):
     assert torch.equal(ops.diff_attention(q, *far, lam, lambda_init=0.3, norm_weight=w), ops.diff_attention(q, k, v, lam, lambda_init=0.3, norm_weight=w))
 
 
+def test_diff_attention_tokens_far_apart(ops):
+    """A cache whose tokens lie 0.7 GB apart: the offsets within one copy of a few tokens pass 32 bits too."""
+    n_k, d, step = 64, 32, 5 << 26
+    cache = torch.empty(step * n_k, dtype=torch.bfloat16, device="cuda")
+    for n_q in (1, 8, 40):
+        q, k, v, lam, w = attention_inputs(9, 1, n_q, n_k, 1, 1, d, torch.bfloat16)
+        far = [cache.as_strided((1, n_k, 1, 2 * d), (0, step, 2 * d, 1), o) for o in (0, 2 * d)]
+        far[0].copy_(k), far[1].copy_(v)
+        assert torch.equal(ops.diff_attention(q, *far, lam, lambda_init=0.3, norm_weight=w), ops.diff_attention(q, k, v, lam, lambda_init=0.3, norm_weight=w)), n_q
+    del cache, far
+    torch.cuda.empty_cache()
+
+
+def test_more_rows_than_one_launch_takes(ops):
+    g = gen(41)
+    n = (1 << 23) + 13
+    q, pos = randn(g, 1, n, 1, 2, dtype=torch.bfloat16), torch.randint(0, 1000, (n,), generator=g, device="cuda")
+    freqs = torch.tensor([0.25], dtype=torch.float64, device="cuda")
+    got = ops.rotary(q, positions=pos, freqs=freqs)
+    for at in (slice(0, 4096), slice(n - 4096, n)):
+        assert torch.equal(got[:, at], ops.rotary(q[:, at], positions=pos[at], freqs=freqs))
+    residual = randn(g, n, 3)
+    pre = ops.Norm(kind="rms")
+    x = ops.residual_norm(residual, pre_norm=pre)[1]
+    for at in (slice(0, 4096), slice((1 << 22) - 50, (1 << 22) + 50), slice(n - 4096, n)):
+        assert torch.equal(x[at], ops.residual_norm(residual[at], pre_norm=pre)[1])
+
+
 # ---- residual norms ------------------------------------------------------------------------------------------------------------
 
 def norm_ref(x, ex, kind, weight, bias, eps):

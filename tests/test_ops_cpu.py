@@ -75,6 +75,13 @@ def test_diff_attention_workspace_and_nothing_to_do(lib):
             assert lib.rz_diff_attention(ctypes.byref(a), 8, need, None) == 10001
 
 
+@pytest.mark.parametrize("many", [{"batch": 1 << 23, "n_q": 1}, {"batch": 1 << 14, "n_q": 1 << 14, "heads": 4, "kv_heads": 4}])
+def test_diff_attention_refuses_more_workgroups_than_a_launch_takes(lib, many):
+    a = attention_args(**many)
+    assert lib.rz_diff_attention_workspace(ctypes.byref(a)) == 0
+    assert lib.rz_diff_attention(ctypes.byref(a), 16, 1 << 40, None) == 10001
+
+
 @pytest.mark.parametrize("same", ["q_dev", "k_dev", "v_dev"])
 def test_diff_attention_does_not_write_over_its_inputs(lib, same):
     a = attention_args(**{**dict(q_dev=1 << 12, k_dev=1 << 13, v_dev=1 << 14), same: 16})
