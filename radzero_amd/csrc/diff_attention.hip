@@ -1295,7 +1295,7 @@ template <typename T, int D, bool KEYS, typename F> Args make(const rz_diff_atte
     x.part_rows = min(x.rows, F::BR);
     x.ws = (float*)ws;
     int equal = 1, ranges = 0;
-    if (tail && (KEYS || !a.causal || !x.full)) {                          // causal rows: after a full round short units are left, whose places free up one by one
+    if (tail && x.blocks && (KEYS || !a.causal || !x.full)) {                          // causal rows: after a full round short units are left, whose places free up one by one
         // a unit has at most 2 + blocks / each pieces
         const int most = min(min(places / tail, x.blocks), kMostSplits);
         if constexpr (KEYS) {

@@ -313,6 +313,8 @@ def test_diff_attention_of_no_keys_and_no_queries(ops):
     q, k = torch.ones(2, 3, 4, 64, device="cuda"), torch.ones(2, 0, 2, 64, device="cuda")
     got = ops.diff_attention(q, k, k, lam, lambda_init=0.2, norm_weight=torch.ones(64, device="cuda"), out=torch.full_like(q, 5.0))
     assert bool((got == 0).all())
+    many = torch.ones(2, 300, 4, 64, device="cuda")
+    assert bool((ops.diff_attention(many, k, k, lam, lambda_init=0.2, out=torch.full_like(many, 5.0)) == 0).all())
     assert ops.diff_attention(q[:, :0], q, q, lam, lambda_init=0.2).shape == (2, 0, 4, 64)
     assert ops.diff_attention(q[:0], q[:0], q[:0], lam, lambda_init=0.2).shape == (0, 3, 4, 64)
 

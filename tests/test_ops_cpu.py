@@ -62,6 +62,18 @@ def test_diff_attention_refuses(lib, bad):
     assert b"rz_diff_attention" in lib.rz_last_error()
 
 
+def test_diff_attention_workspace_of_any_sizes(lib):
+    """No keys, one key, one block too few or too many: the plan of the work comes out, and what it stores stays within what fills the chip once."""
+    for dtype in (0, 1):
+        for head_dim in (32, 64, 128):
+            for n_q in (1, 2, 3, 5, 33, 200, 5000):
+                for n_k in (0, 1, 63, 64, 65, 1000, 1 << 16, 1 << 30):
+                    for batch, lens in ((1, None), (3, 16), (64, 16), (65, 16), (700, None)):
+                        for causal in (0, 2):
+                            a = attention_args(dtype=dtype, head_dim=head_dim, n_q=n_q, n_k=n_k, batch=batch, kv_lens_dev=lens, causal=causal)
+                            assert lib.rz_diff_attention_workspace(ctypes.byref(a)) <= 2048 * 128 * (4 * head_dim + 4) * 4
+
+
 def test_diff_attention_workspace_and_nothing_to_do(lib):
     assert lib.rz_diff_attention(None, None, 0, None) == 10001
     assert lib.rz_diff_attention(ctypes.byref(attention_args(n_q=0)), None, 0, None) == 0
