@@ -62,9 +62,15 @@ def _vector(x, name, shape, device):
     return x.data_ptr()
 
 
+_empty_like = torch.empty_like
+
+
+def _new(like):
+    """A contiguous tensor of this one's shape, type and device, the cheapest way (empty_like would keep other strides too)."""
+    return _empty_like(like) if like.is_contiguous() else like.new_empty(tuple(like.shape))
+
+
 def _output(out, like_shape, dtype, device, name):
-    if out is None:
-        return torch.empty(like_shape, dtype=dtype, device=device)
     _need(isinstance(out, torch.Tensor) and out.shape == like_shape and out.dtype == dtype and out.device == device,
           f"{name} must be {dtype} {tuple(like_shape)} on {device}")
     _need(all(s for s, n in zip(out.stride(), out.shape) if n > 1) and (out.stride(-1) == 1 or out.shape[-1] == 1), f"{name}: columns must be contiguous, rows apart")
@@ -165,12 +171,11 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torc
         shape, strides = shape[:-1], strides[:-1]
     _need(shape == (b, n) or shape == (n,), "positions must be (tokens,) or (batch, tokens)")
     if out is None:
-        qo = torch.empty((b, n, hq, d), dtype=dt, device=dev)
-        ko = torch.empty((b, n, hk, d), dtype=dt, device=dev) if k is not None else None
+        qo, ko = _new(q), None if k is None else _new(k)
     else:
         qo, ko = (out, None) if k is None else out
-        qo = _output(qo, q.shape, dt, dev, "out")
-        ko = None if k is None else _output(ko, k.shape, dt, dev, "out")
+        qo = _new(q) if qo is None else _output(qo, q.shape, dt, dev, "out")
+        ko = None if k is None else _new(k) if ko is None else _output(ko, k.shape, dt, dev, "out")
     kos, kp, kop = ks, 0, 0
     if hk:
         ks, kos, kp, kop = k.stride(), ko.stride(), k.data_ptr(), ko.data_ptr()
@@ -226,14 +231,14 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
         if n_k > 1 and x.stride(1) != 1:
             x = x.contiguous()
         attention_mask, mask, mask_stride = x, x.data_ptr(), x.stride(0)
-    out = torch.empty((b, n_q, h, w), dtype=dt, device=dev) if out is None else _output(out, q.shape, dt, dev, "out")
+    out = _new(q) if out is None else _output(out, q.shape, dt, dev, "out")
     os = out.stride()
     args = _lib.RzDiffAttentionArgs.pack(
         _DTYPES[dt], b, h, hk, n_q, n_k, d, _CAUSAL[causal], d ** -0.5 if scale is None else scale, lambda_init, norm_eps, out_scale,
         q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], out.data_ptr(), os[0], os[1], os[2],
         lam, 4 * d if per_head else 0, _vector(norm_weight, "norm_weight", (w,), dev), lens, mask, mask_stride)
     need = _fn("rz_diff_attention_workspace")(args)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _call("rz_diff_attention", _WORKSPACE_STREAM, dev, args, ws.data_ptr() if need else 0, need)
     return out
 
@@ -277,7 +282,7 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
     ro, xo = (None, None) if out is None else out
     rp, rs, xp, xs = 0, (0, 0, 0), 0, (0, 0, 0)
     if y is not None or alpha != 1.0 or ro is not None or pre_norm is None:
-        ro = torch.empty(shape, dtype=rt, device=dev) if ro is None else _output(ro, shape, rt, dev, "out[0]")
+        ro = _new(residual) if ro is None else _output(ro, shape, rt, dev, "out[0]")
         rp, rs = ro.data_ptr(), ro.stride()
     else:
         ro = residual
@@ -290,7 +295,7 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
         pre_w, pre_b, pre_eps, pre_kind = pre_norm
         _need(pre_kind in _NORM, "pre_norm.kind must be layer or rms")
         pre_kind, pre_w, pre_b = _NORM[pre_kind], _vector(pre_w, "pre_norm.weight", (dim,), dev), _vector(pre_b, "pre_norm.bias", (dim,), dev)
-        xo = torch.empty(shape, dtype=t, device=dev) if xo is None else _output(xo, shape, t, dev, "out[1]")
+        xo = _output(xo, shape, t, dev, "out[1]") if xo is not None else _new(residual) if rt is t else _new(y) if y is not None else residual.new_empty(tuple(shape), dtype=t)
         xp, xs = xo.data_ptr(), xo.stride()
     else:
         _need(xo is None, "out[1] needs pre_norm")
