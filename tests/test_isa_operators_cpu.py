@@ -49,9 +49,13 @@ def functions(tmp_path_factory):
 
 def registers(operands):
     out = set()
-    for kind, a, b, kind1, n in re.findall(r"\b(?:([va])\[(\d+):(\d+)\]|([va])(\d+))\b", operands):
+    for kind, a, b, kind1, n in re.findall(r"\b(?:([va])\[(\d+):(\d+)\]|([va])(\d+)\b)", operands):
         out.update((kind, i) for i in range(int(a), int(b) + 1)) if kind else out.add((kind1, int(n)))
     return out
+
+
+def test_registers():
+    assert registers("v[2:3], v7, -v208, s[40:41], a[0:1], 0") == {("v", 2), ("v", 3), ("v", 7), ("v", 208), ("a", 0), ("a", 1)}
 
 
 def test_no_packed_fp32(functions):
