@@ -25,7 +25,10 @@ if EXPERIMENTS:
     # generated loops attention.hip's and gemm10.hip's experiment branches include) and are found through -I
     SOURCES += ["gemm10.hip", "gemm11.hip", "gemm12.hip"]
 # attention.hip: fmaxf chains on MFMA outputs fuse into v_max3_f32 without a canonicalising v_max each
-EXTRA_FLAGS = {"attention.hip": ["-fno-honor-nans"]}
+EXTRA_FLAGS = {"attention.hip": ["-fno-honor-nans"],
+               # results of matrix instructions in ordinary registers wherever they fit: the fp32 kernels' vector instructions work on them, and every one in an
+               # accumulation register costs a move each way (one block of 32 keys of head dim 64: 573 -> 421 vector instructions)
+               "diff_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # no packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): hipcc -O3 makes it from ordinary float code, and on these machines some of its

@@ -440,22 +440,37 @@ template <typename T, int D, int MAPS, int PLANES> struct Wave {             // 
 #pragma unroll
                     for (int y = 0; y < MAPS; ++y) o[y][cb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[y].w[e], o[y][cb], 0, 0, 0);
                 }
+        } else if constexpr (PLANES == 3) {
+            // the 32 keys' products are summed by themselves and join O once: 12 roundings at the size of O for every 32 keys would cost a decimal over 3500 keys
+#pragma unroll
+            for (int cb = 0; cb < NC; ++cb) {
+                f32x16 t[MAPS] = {};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t at = (vt ^ ((cb & 3) << 6)) + (cb >> 2) * 256 + 16 * u * RB;
+                    chunk v[3];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) v[i] = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at + i * PLANE), tr(at + i * PLANE + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int y = 0; y < MAPS; ++y) {
+                        const chunk w[3] = {p[y].w[0][u], p[y].w[1][u], p[y].w[2][u]};
+                        t[y] = mma(v, w, t[y]);
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < MAPS; ++y)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[y][cb][e] += t[y][e];
+            }
         } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int cb = 0; cb < NC; ++cb) {
                     const uint32_t at = (vt ^ ((cb & 3) << 6)) + (cb >> 2) * 256 + 16 * u * RB;
-                    chunk v[PLANES];
+                    const chunk v = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at), tr(at + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int i = 0; i < PLANES; ++i) v[i] = __builtin_bit_cast(chunk, __builtin_shufflevector(tr(at + i * PLANE), tr(at + i * PLANE + 8 * RB), 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int y = 0; y < MAPS; ++y) {
-                        chunk w[PLANES];
-#pragma unroll
-                        for (int i = 0; i < PLANES; ++i) w[i] = p[y].w[i][u];
-                        o[y][cb] = mma(v, w, o[y][cb]);
-                    }
+                    for (int y = 0; y < MAPS; ++y) o[y][cb] = Op<T>::mma(v, p[y].w[0][u], o[y][cb]);
                 }
         }
     }
@@ -784,6 +799,18 @@ __global__ __launch_bounds__(64 * F::W, F::kWaves) void diff_attention_kernel(co
 #pragma unroll
                     for (int w = 0; w < W; ++w) odd |= (uint32_t)scalar((int)odd_keys_of[w]);
                 __builtin_amdgcn_sched_barrier(0);
+                if constexpr (live) {                                     // the queries, operands of products alone, where only those reach: the vector unit works on O
+#pragma unroll
+                    for (int k = 0; k < PLANES; ++k)
+#pragma unroll
+                        for (int y = 0; y < MAPS; ++y)
+#pragma unroll
+                            for (int t = 0; t < S::NT; ++t) asm volatile("" : "+a"(wv.q[k][y][t]));
+#pragma unroll
+                    for (int y = 0; y < MAPS; ++y)
+#pragma unroll
+                        for (int cb = 0; cb < NC; ++cb) asm volatile("" : "+v"(wv.o[y][cb]));
+                }
                 if constexpr (live) wv.block(lds_address(lds) + k_at, lds_address(lds) + v_at, bits, lim - j, bits == ~0u && j + BN <= wave_first, odd);
             }
         };
@@ -1266,8 +1293,8 @@ template <int D> bool keys_form(int64_t rows) { return D <= 64 && rows <= 32; }
 // What the ways to run the last round cost, in microseconds: its longest workgroup, the partial results written and read again (5 TB/s), the join's launch.  A block of
 // 64 keys takes a workgroup `alone` on its CU, or beside one or two others, as long as measured here with 256 of them on every CU, 1024 and 2048 keys.
 template <typename T, int D> struct Cost {
-    static constexpr double alone = sizeof(T) == 4 ? (D == 32 ? 4.75 : D == 64 ? 8.2 : 10.1) : D == 32 ? 1.65 : D == 64 ? 2.24 : 3.07;
-    static constexpr double beside = sizeof(T) == 4 ? (D == 32 ? 3.2 : 0.) : D == 32 ? 0.69 : D == 64 ? 0.82 : 0.29;
+    static constexpr double alone = sizeof(T) == 4 ? (D == 32 ? 4.75 : D == 64 ? 8.4 : 10.4) : D == 32 ? 1.65 : D == 64 ? 2.24 : 3.07;
+    static constexpr double beside = sizeof(T) == 4 ? (D == 32 ? 3.7 : 0.) : D == 32 ? 0.69 : D == 64 ? 0.82 : 0.29;
     static constexpr double join = 5., second = 3.;            // a stretch over two units starts and ends twice
     static double run(int blocks, int64_t groups) { return blocks * (alone + beside * (double)((groups - 1) / cu_count())); }
     static double pieces(int64_t n, int rows) { return n * (rows * (4. * D * sizeof(float)) * 2 / 5e6); }

@@ -206,6 +206,16 @@ def test_diff_attention_longer(ops, dtype, shape):
     assert torch.equal(got, ops.diff_attention(q, k, v, lam, lambda_init=0.4, norm_weight=w)), "two calls differ"
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_diff_attention_fp32_over_many_keys(ops, d):
+    """The root mean square error of fp32 over 3500 keys.  32 keys' products join O at a time, n_k / 32 roundings of at most half a step at O's size, which go either way:
+    sqrt(n_k / 32) of them; as much again for the weights and their sums."""
+    q, k, v, lam, _ = attention_inputs(23, 1, 300, 3500, 4, 2, d, torch.float32, std=1.0)
+    got = ops.diff_attention(q, k, v, lam, lambda_init=0.3).double()
+    ref, _ = attention_ref(q, k, v, lam, 0.3)
+    assert float((got - ref).square().sum().sqrt() / ref.square().sum().sqrt()) <= math.sqrt(2) * math.sqrt(3500 / 32) * E
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("causal", [None, "start", "end"])
 @pytest.mark.parametrize("keys", ["all", "lens", "mask", "both"])
