@@ -457,7 +457,7 @@ def test_residual_norm_views_in_place_and_neighbours(ops, dtype):
     assert r.shape == (b, 0, d) and x.shape == (b, 0, d)
 
 
-@pytest.mark.parametrize("d", [64, 190, 768, 1024], ids=str)
+@pytest.mark.parametrize("d", [1, 3, 16, 17, 64, 65, 128, 129, 190, 193, 256, 257, 385, 512, 513, 768, 769, 1024, 1025], ids=str)
 def test_residual_norm_many_rows(ops, d):
     """More rows than waves, so that a wave takes several, with runs that cross from one sample to the next: each sample's own gate, a gate per row, in place."""
     g = gen(35 + d)
