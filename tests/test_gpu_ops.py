@@ -78,6 +78,14 @@ def test_rotary(ops, dtype, case, layout):
             close(y, *rotary_ref(x, pos, table, layout, amplitude), "rotary")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("case", [(2, 19, 3, 1, 70, 70, 1, 1000), (3, 40, 2, 2, 46, 28, 1, 1000), (1, 9, 5, 1, 12, 12, 3, 30), (1, 300, 4, 4, 26, 20, 1, 500)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_of_pairs(ops, dtype, case, layout):
+    """Widths that divide by two and no further."""
+    test_rotary(ops, dtype, case, layout)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 def test_rotary_views_shared_positions_and_in_place(ops, dtype, layout):
