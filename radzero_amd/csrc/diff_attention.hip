@@ -1014,7 +1014,7 @@ template <typename T, int D> __device__ __forceinline__ void finish_row(const Ar
     for (int e = 0; e < N; ++e) out[e] = from_f32<T>(o[0][e] * f * (a.norm_weight_dev ? a.norm_weight_dev[lane * N + e] : 1.f));
 }
 
-// Few query rows (R at most) over many keys, bound by HBM: no matrix unit, whose 32 columns would stay empty.  D / 4 lanes take a key, 8 of its columns each: half of
+// Few query rows (R at a time) over many keys, bound by HBM: no matrix unit, whose 32 columns would stay empty.  D / 4 lanes take a key, 8 of its columns each: half of
 // them the first map's, half the second's; 256 / D keys of a wave at a time, kFly such steps on their way.  Every place of a key keeps its own maxima, sums and O of all rows;
 // they meet at the end, in the wave, then in LDS.  Weights stay fp32.
 template <typename T, int D, int R> struct Few {
@@ -1065,7 +1065,8 @@ template <typename T, int D, int R> __global__ __launch_bounds__(256, (Few<T, D,
     if (!at.any) return;
     const int shift = a.causal == RZ_CAUSAL_END ? at.n - a.n_q : 0;
     auto limit = [&](int row) -> int { return a.causal ? min(at.n, scalar(row / x.group) + 1 + shift) : at.n; };
-    const int end = max(limit(x.rows - 1), 0), first = limit(0);           // keys of the last row, of all rows
+    const int row0 = at.rb * R, rows = min(R, x.rows - row0);
+    const int end = max(limit(row0 + rows - 1), 0), first = limit(row0);   // keys of the last row, of all rows
     const bool whole = at.lo == 0 && at.hi == at.of;
     const int begin = whole ? 0 : at.key(at.lo, end), stop = whole ? end : at.key(at.hi, end);
 
@@ -1077,7 +1078,7 @@ template <typename T, int D, int R> __global__ __launch_bounds__(256, (Few<T, D,
     int lim[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int rr = min(r, x.rows - 1), i = scalar(rr / x.group), head = at.hk * x.group + rr - i * x.group;
+        const int rr = row0 + min(r, rows - 1), i = scalar(rr / x.group), head = at.hk * x.group + rr - i * x.group;
         Eight<T> e;
         e.load((const T*)a.q_dev + at.b * a.q_batch_stride + i * a.q_token_stride + head * a.q_head_stride + col);
         e.get(q[r]);
@@ -1185,7 +1186,7 @@ template <typename T, int D, int R> __global__ __launch_bounds__(256, (Few<T, D,
             }
     }
     __syncthreads();
-    for (int r = wave; r < x.rows; r += W) {
+    for (int r = wave; r < rows; r += W) {
         f32x4 st[W];
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, t[2][N] = {};
 #pragma unroll
@@ -1204,7 +1205,7 @@ template <typename T, int D, int R> __global__ __launch_bounds__(256, (Few<T, D,
             }
         }
         if (whole) {
-            const int i = scalar(r / x.group), head = at.hk * x.group + r - i * x.group;
+            const int i = scalar((row0 + r) / x.group), head = at.hk * x.group + row0 + r - i * x.group;
             finish_row<T, D>(x, t, l0, l1, head_lambda(a, a.lambda_head_stride ? head : 0, lane), at.b, i, head, lane);
         } else {
             const int64_t slot = (int64_t)at.slot * x.part_rows + r;
@@ -1283,9 +1284,10 @@ int cu_count() {
 }
 
 // Hardly any rows: no matrix unit.  us, with it / without, head dim 64: bf16, one row, 1 x 6 heads over 257 keys 12.8 / 10.4, 64 x 12 over 300 42 / 24; two rows 43 / 26, but
-// 8 x 4 over 300 12.8 / 15.7: only where every CU has a unit; four rows 43 / 56.  fp32, four rows, 8 x 4 over 8192 120 / 55.
-template <typename T> bool few_form(const rz_diff_attention_args& a, int64_t rows) {
-    return rows <= (sizeof(T) == 4 ? 4 : 1) || (rows == 2 && (int64_t)a.batch * a.kv_heads >= cu_count());
+// 8 x 4 over 300 12.8 / 15.7: only where every CU has a unit; four rows 43 / 56.  fp32, four rows, 8 x 4 over 8192 120 / 55;
+// eight (two blocks of four, each key read twice, by the same XCD), 64 x 12 over 300, head dims 32, 64, 128 60 / 68, 131 / 93, 215 / 197; twelve 60 / 104, 131 / 132, 216 / 240.
+template <typename T, int D> bool few_form(const rz_diff_attention_args& a, int64_t rows) {
+    return rows <= (sizeof(T) == 4 ? (D == 32 ? 4 : 8) : 1) || (rows == 2 && (int64_t)a.batch * a.kv_heads >= cu_count());
 }
 // Few rows: the waves of a workgroup share the rows and split the keys (head dims 32 and 64).
 template <int D> bool keys_form(int64_t rows) { return D <= 64 && rows <= 32; }
@@ -1372,7 +1374,7 @@ template <typename T, int D, bool KEYS, typename F> hipError_t launch(void (*k)(
 // One of the forms for these sizes: use(KEYS, form, kernel).
 template <typename T, int D, typename Use> auto with_form(const rz_diff_attention_args& a, Use use) {
     const int64_t rows = (int64_t)a.n_q * (a.heads / a.kv_heads);
-    if (few_form<T>(a, rows)) {
+    if (few_form<T, D>(a, rows)) {
         if (rows == 1) return use(std::true_type{}, Few<T, D, 1>{}, diff_attention_few_kernel<T, D, 1>);
         if (rows == 2) return use(std::true_type{}, Few<T, D, 2>{}, diff_attention_few_kernel<T, D, 2>);
         if constexpr (sizeof(T) == 4) return use(std::true_type{}, Few<T, D, 4>{}, diff_attention_few_kernel<T, D, 4>);

@@ -264,6 +264,24 @@ def test_diff_attention_very_unequal_lengths(ops, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("shape", [(1, 5, 1), (2, 4, 1), (3, 4, 2), (8, 2, 2), (7, 1, 1), (3, 1, 1), (1, 4, 2)], ids=str)
+def test_diff_attention_few_rows(ops, dtype, d, shape):
+    """One to eight query rows of a key head, the last block of them not full: causal edges inside a block, lengths, holes, and NaN under every hidden key."""
+    n_q, h, hk = shape
+    b, n_k = 4, 777
+    q, k, v, lam, w = attention_inputs(n_q * 100 + h + d, b, n_q, n_k, h, hk, d, dtype)
+    lens = torch.tensor([n_k, n_q + 1, 0, 500], dtype=torch.int32, device="cuda")
+    mask = (torch.rand(b, n_k, generator=gen(5), device="cuda") < 0.6).long()
+    for causal in (None, "start", "end"):
+        for m in (None, mask):
+            used = seen_keys(b, n_q, n_k, causal, lens, m).any(1)[..., None, None]
+            bad_k, bad_v = torch.where(used, k, math.nan), torch.where(used, v, math.inf)
+            got = ops.diff_attention(q, bad_k.to(dtype), bad_v.to(dtype), lam, lambda_init=0.3, causal=causal, kv_lens=lens, attention_mask=m, norm_weight=w)
+            close(got, *attention_ref(q, k, v, lam, 0.3, causal=causal, lens=lens, mask=m, norm=w))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("causal", ["start", "end"])
 def test_diff_attention_causal_over_several_rounds(ops, dtype, causal):
     """More blocks of query rows than the chip holds at a time, each row written once whatever the order they run in."""
