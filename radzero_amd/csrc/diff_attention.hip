@@ -680,8 +680,9 @@ template <typename T, int D> struct Out {
     }
 };
 
-__device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, float sum_of_squares) {
-    return a.norm_weight_dev ? a.out_scale / sqrtf(sum_of_squares / (float)(2 * a.head_dim) + a.norm_eps) : a.out_scale;
+// `l`: either map's sum of weights, 0 where the query sees no key.  Such a row is all zeros, and stays so where an eps of 0 would make its factor infinite.
+__device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, float sum_of_squares, float l) {
+    return !a.norm_weight_dev ? a.out_scale : l == 0.f ? 0.f : a.out_scale / sqrtf(sum_of_squares / (float)(2 * a.head_dim) + a.norm_eps);
 }
 
 template <typename T, int D, bool KEYS, typename F = Form<T, D, KEYS>>
@@ -992,7 +993,7 @@ __global__ __launch_bounds__(64 * F::W, F::kWaves) void diff_attention_kernel(co
         ss = 0.f;
         for (int w = 0; w < W; ++w) ss += stat[w * 32 + (lane & 31)];
     }
-    Out<T, D>::template store<OSTEP, OWN>(x, o[0], own0, at.b, i, head, live, norm_factor(a, ss), h);
+    Out<T, D>::template store<OSTEP, OWN>(x, o[0], own0, at.b, i, head, live, norm_factor(a, ss, l[0]), h);
     return;                                                                // a whole unit is a workgroup's only piece
     }
 }
@@ -1008,7 +1009,7 @@ template <typename T, int D> __device__ __forceinline__ void finish_row(const Ar
         o[0][e] = o[0][e] * r0 - o[1][e] * r1;
         ss = fmaf(o[0][e], o[0][e], ss);
     }
-    const float f = norm_factor(a, wave_sum(ss));
+    const float f = norm_factor(a, wave_sum(ss), l0);
     T* out = (T*)a.out_dev + b * a.out_batch_stride + i * a.out_token_stride + head * a.out_head_stride + lane * N;
 #pragma unroll
     for (int e = 0; e < N; ++e) out[e] = from_f32<T>(o[0][e] * f * (a.norm_weight_dev ? a.norm_weight_dev[lane * N + e] : 1.f));

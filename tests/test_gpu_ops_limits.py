@@ -1,0 +1,53 @@
+"""The operators' calls at the ends of what their documentation allows, against their definitions in 64 bits: norms without an eps, weights and positions at the ends of their
+types' ranges, long sums, outputs that share memory with inputs."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["f32", "bf16", "f16"]
+U = {t: torch.finfo(t).eps / 2 for t in TYPES}
+E = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need a HIP device"
+    from radzero_amd import ops
+    return ops
+
+
+def randn(seed, *shape, std=1.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda") * std).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("shape", [(1, 300), (8, 300), (20, 300), (200, 300), (1, 9000), (3, 9000), (20, 9000), (200, 9000)], ids=str)
+def test_diff_attention_of_hidden_rows_without_an_eps(ops, dtype, d, shape):
+    """norm_eps = 0: a query that sees no key still gets zeros (an empty sequence, a mask of nothing, causal rows before the first key), whole and in pieces; the others what
+    an eps far below their mean square gives, and NaN stays NaN."""
+    n_q, n_k = shape
+    b, h = 4, 2
+    q, k, v = randn(1, b, n_q, h, 2 * d, dtype=dtype), randn(2, b, n_k, h, 2 * d, dtype=dtype), randn(3, b, n_k, h, 2 * d, dtype=dtype) + 1
+    lam, w = torch.zeros(4, d, device="cuda"), torch.ones(2 * d, device="cuda")
+    mask = torch.ones(b, n_k, dtype=torch.int64, device="cuda")
+    mask[1] = 0
+    lens = torch.tensor([0, n_k, n_q // 2, n_k], dtype=torch.int32, device="cuda")
+    for kv_lens in (None, lens):
+        for causal in (None, "end"):
+            call = lambda eps: ops.diff_attention(q, k, v, lam, lambda_init=0.3, causal=causal, kv_lens=kv_lens, attention_mask=mask, norm_weight=w, norm_eps=eps)      # noqa: E731
+            got = call(0.0)
+            n = torch.full((b,), n_k, device="cuda") if kv_lens is None else kv_lens.long()
+            n[1] = 0
+            sees = (n[:, None] > 0) & ((n[:, None] - n_q + torch.arange(n_q, device="cuda") >= 0) if causal else torch.ones(1, n_q, dtype=torch.bool, device="cuda"))
+            assert bool((got[~sees] == 0).all()), (kv_lens is not None, causal)
+            assert bool(torch.isfinite(got.float()).all())
+            # a mean square is at least 1e-6 here (values of mean 1, 1 - lambda = 0.7): 1e-30 beside it changes nothing
+            assert torch.equal(got, call(1e-30))
+    k[3, 0, 0, 0] = math.nan
+    got = ops.diff_attention(q, k, v, lam, lambda_init=0.3, attention_mask=mask, norm_weight=w, norm_eps=0.0)
+    assert bool(got[3, :, 0].isnan().all()) and bool((got[1] == 0).all()) and bool(torch.isfinite(got[3, :, 1].float()).all())
