@@ -263,8 +263,9 @@ int rz_rotary(const rz_rotary_args* args, void* stream);
  *   (batch, n_k), 0 = hidden, NULL = none (the tokenizer's attention_mask as it comes); causal RZ_CAUSAL_START: query i is token i and sees keys
  *   0 .. i; RZ_CAUSAL_END: the queries are the last n_q tokens of their sequence, query i sees keys 0 .. len - n_q + i.  A query that sees no key
  *   gets zeros.  What a hidden key holds, inf and NaN included, changes nothing.
- *   Statistics and sums are fp32; the 16-bit types round each weight exp(s - max) to the type for the product with v.  fp32 products may be taken
- *   from three bf16 parts of each operand (2^-22 |a||b| off); an infinity where a query sees it gives NaN.  out must not overlap the inputs.
+ *   Statistics and sums are fp32; the 16-bit types round each weight exp(s - max) to the type for the product with v (f16, whose steps end: weights too
+ *   small for it lose at most 2^-13 of a row's sum together, over up to 2^22 keys).  fp32 products may be taken from three bf16 parts
+ *   of each operand (2^-22 |a||b| off); an infinity where a query sees it gives NaN.  out must not overlap the inputs.
  *   workspace_dev: rz_diff_attention_workspace(args) bytes (0: may be NULL), 16-byte aligned, free for reuse when the call's kernels are done. */
 enum rz_causal { RZ_CAUSAL_NONE = 0, RZ_CAUSAL_START = 1, RZ_CAUSAL_END = 2 };
 typedef struct rz_diff_attention_args {

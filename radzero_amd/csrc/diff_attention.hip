@@ -186,7 +186,7 @@ struct Args {
     int blocks, ranges, each, more;                            // blocks of a unit, of 64 keys (keys form: as many as it has pieces); a workgroup's stretch: `each`, one more for the first `more` of them
     bool shared;
     int splits, least;                                         // shared: pieces of a unit on average, keys of a piece at least
-    float c;                                                   // scale * log2(e)
+    float c, up;                                               // scale * log2(e); f16_up
     int part_rows, slots;                                      // rows of a unit in the workspace, its places for pieces
     float* ws;
 };
@@ -301,6 +301,16 @@ __device__ __forceinline__ float head_lambda(const rz_diff_attention_args& a, in
     return expf(wave_sum(x1)) - expf(wave_sum(x2)) + a.lambda_init;
 }
 
+// Steps of f16 end at 2^-24: what a smaller weight is rounded by, 2^-25 at most, is lost alike for all keys of a flat tail (65535 keys of weight 2^-25.05 beside one of 1: all of
+// their 1.9e-3 of the sum).  The weight of a row's first reference is 2^up, so that n keys lose 2^(log2 n - 25 - up) = 2^-13 of its sum at most, a quarter of the rounding of the
+// result; what is left of 2^16 is for maxima that grow.  Up to 4096 keys: 0.  10 at most: beyond 2^22 keys of one wave, n 2^-35.
+// A constant 8 would cost rows whose scores spread widely more turns of the slow path (8 x 1370 tokens, 6 heads of 64, scores of deviation 4.5: 112 -> 144 us).
+inline float f16_up(int n_k) {
+    int up = 0;
+    while (up < 10 && n_k > 4096 << up) ++up;
+    return (float)up;
+}
+
 // bits of the keys below `n` (any n)
 __device__ __forceinline__ uint64_t below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
@@ -314,13 +324,14 @@ template <typename T, int D, int MAPS, int PLANES> struct Wave {             // 
 
     chunk q[PLANES][MAPS][NT];
     f32x16 o[MAPS][NC];
-    float m[MAPS], l[MAPS];                 // reference maximum of the scores in log2 units (-inf: no key yet), this lane's share of the sum
+    float m[MAPS], l[MAPS];                 // reference of the scores in log2 units: their maximum so far or an earlier one, less `up` (-inf: no key yet), this lane's share of the sum
     float c;                          // scale * log2(e)
+    float up;                         // f16: the key of the reference has weight 2^up
     int h;                            // which half of every 8 keys the lane holds
     bool started;                     // every row has a reference maximum (wave-uniform)
 
     template <typename Q> __device__ __forceinline__ void init(const Args& x, const Q* qrow) {      // qrow: the first of the wave's maps
-        c = x.c;
+        c = x.c, up = std::is_same<T, f16_t>::value ? x.up : 0.f;
         started = false;
 #pragma unroll
         for (int y = 0; y < MAPS; ++y) {
@@ -377,7 +388,7 @@ template <typename T, int D, int MAPS, int PLANES> struct Wave {             // 
             s[e] = (seen >> (8 * (e / 4) + e % 4)) & 1 ? s[e] : -INFINITY;
             mx = fmaxf(mx, s[e]);
         }
-        const float top = pair_max(mx) * c, mn = need ? fmaxf(m[y], top) : m[y];
+        const float top = pair_max(mx) * c - up, mn = need ? fmaxf(m[y], top) : m[y];
         if (__any(mn > m[y])) {
             const float f = m[y] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[y] - mn);            // m == mn: 1
             l[y] *= f;
@@ -398,9 +409,10 @@ template <typename T, int D, int MAPS, int PLANES> struct Wave {             // 
 #pragma unroll
         for (int e = 0; e < 16; ++e) p[e] = __uint_as_float(__float_as_uint(p[e]) & (uint32_t)__builtin_amdgcn_sbfe((int)seen, 8 * (e / 4) + e % 4, 1));
     }
-    // The weights of 32 keys without a maximum: one that outgrows the reference shows in the sum.  2^15 keeps every weight below the largest f16.  False: some row's did.
+    // The weights of 32 keys without a maximum: one that outgrows the reference shows in the sum, which 16 finite weights of f16 keep below 2^20 (rounding one beyond 65504
+    // gives an infinity).  False: some row's did.
     // One run of instructions from the matrix products to what reads them: with a branch between, the fp32 kernels came out without the wait states they need.
-    static constexpr float kMost = 32768.f;
+    static constexpr float kMost = std::is_same<T, f16_t>::value ? 1048576.f : 32768.f;
     template <bool HIDE> __device__ __forceinline__ bool straight(uint32_t kt, uint32_t seen, W (&p)[MAPS], float (&t)[MAPS], bool& fine) const {
         f32x16 s[MAPS];
 #pragma unroll
@@ -1311,6 +1323,7 @@ template <typename T, int D, bool KEYS, typename F> Args make(const rz_diff_atte
     Args x;
     x.a = a;
     x.c = a.scale * 1.44269504088896340736f;
+    x.up = f16_up(a.n_k);
     x.group = a.heads / a.kv_heads;
     x.rows = a.n_q * x.group;
     x.row_blocks = (x.rows + F::BR - 1) / F::BR;

@@ -196,7 +196,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
     causal: "start" = query i is token i and sees keys 0 .. i; "end" = the queries are the last n_q tokens of their sequence.
     kv_lens integer (batch,): only the first kv_lens[b] keys count.  attention_mask (batch, n_k): 0 = hidden, as a tokenizer gives it.  A query that sees
     no key gets zeros; what hidden keys hold changes nothing.  norm_weight float32 (2 d): root-mean-square norm of every head's output.
-    Sums and statistics are float32; the 16-bit types round each weight for the product with v; float32 products may be taken from three bf16 parts of each
+    Sums and statistics are float32; the 16-bit types round each weight for the product with v (float16: weights too small for it lose at most 2^-13 of
+    a row's sum together, over up to 2^22 keys); float32 products may be taken from three bf16 parts of each
     operand (2^-22 of |a||b| off; an infinity that a query sees then gives NaN).
     16-byte alignment of q, k, v and out and of their strides is required.  Returns (batch, n_q, heads, 2 d), in `out` (no input's memory) if given."""
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES and q.dim() == 4 and not q.requires_grad):

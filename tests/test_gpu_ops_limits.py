@@ -51,3 +51,31 @@ def test_diff_attention_of_hidden_rows_without_an_eps(ops, dtype, d, shape):
     k[3, 0, 0, 0] = math.nan
     got = ops.diff_attention(q, k, v, lam, lambda_init=0.3, attention_mask=mask, norm_weight=w, norm_eps=0.0)
     assert bool(got[3, :, 0].isnan().all()) and bool((got[1] == 0).all()) and bool(torch.isfinite(got[3, :, 1].float()).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("at", [0, 30000, 65535])
+@pytest.mark.parametrize("below", [20.03, 25.05, 28.0])
+@pytest.mark.parametrize("shape", [(512, 3), (600, 64)], ids=str)
+def test_diff_attention_one_key_above_a_flat_tail(ops, dtype, at, below, shape):
+    """One key, and 65535 whose weights are 2^-below of its own each: their share of the sum is kept, whether a query's keys are in one piece or several.
+
+    Bounds.  A weight is rounded by at most u of it, or, in f16, whose steps end at 2^-24, by 2^-25 on a scale that puts the largest weight at 2^4 or above for 65536 keys:
+    2^16 2^-29 = 2^-13 of the sum.  That and the sum's own rounding (n / 16 additions of fp32 at worst) count in the values' sum and in the weights' sum: twice.  The scores'
+    exponents are below 32 and off by 2 E of them."""
+    units, n_q = shape
+    d, n = 64, 1 << 16
+    q, k, v = (torch.zeros(x, 1, 2 * d, device="cuda", dtype=dtype) for x in (n_q, n, n))
+    q[:, 0, 0] = 8
+    k[at, 0, 0] = below * math.log(2)
+    v[:] = 1
+    v[at, 0, :32], v[:, 0, 32:64] = 0, 0
+    v[at, 0, 32:64] = 1
+    got = ops.diff_attention(*(x.expand(units, -1, -1, -1) for x in (q, k, v)), torch.zeros(4, d, device="cuda"), lambda_init=0.0, scale=1 / 8).double()
+    tail = (n - 1) * math.exp(-float(k[at, 0, 0].double()))
+    head, tail = 1 / (1 + tail), tail / (1 + tail)
+    u = U[dtype] if dtype != torch.float32 else 0.0
+    for columns, ref in ((slice(0, 32), tail), (slice(32, 64), head), (slice(64, 128), 1.0)):
+        off = 2 * (u * tail + (2.0 ** -13 if dtype == torch.float16 else 0)) if ref != 1.0 else 0
+        tol = off + 2 * n / 16 * E * ref + 128 * E * tail + U[dtype] * ref + 2.0 ** -25
+        assert float((got[..., columns] - ref).abs().max()) <= tol, (columns, ref, got[..., columns].min(), got[..., columns].max(), tol)
