@@ -79,3 +79,31 @@ def test_diff_attention_one_key_above_a_flat_tail(ops, dtype, at, below, shape):
         off = 2 * (u * tail + (2.0 ** -13 if dtype == torch.float16 else 0)) if ref != 1.0 else 0
         tol = off + 2 * n / 16 * E * ref + 128 * E * tail + U[dtype] * ref + 2.0 ** -25
         assert float((got[..., columns] - ref).abs().max()) <= tol, (columns, ref, got[..., columns].min(), got[..., columns].max(), tol)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 4, 8, 12, 32, 70])
+def test_diff_attention_fp32_of_equal_values(ops, d, rows):
+    """65536 equal scores (every weight is 1) and equal values of 1 + 2^-12, keys not split over workgroups: the mean is the value.
+
+    Whatever the sums' size, a form may round them once for 32 keys, by half a step at most: n / 32 times E of the result, if every rounding went the same way.  Adding fewer keys
+    at a time does that here: the value's last bit falls off the sum each time."""
+    n, units, value = 1 << 16, 1100, 1 + 2.0 ** -12
+    q, k, v = torch.zeros(1, rows, 1, 2 * d, device="cuda"), torch.zeros(1, n, 1, 2 * d, device="cuda"), torch.full((1, n, 1, 2 * d), value, device="cuda")
+    got = ops.diff_attention(*(x.expand(units, -1, -1, -1) for x in (q, k, v)), torch.zeros(4, d, device="cuda"), lambda_init=0.0)
+    assert float((got.double() / value - 1).abs().max()) <= n / 32 * E
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 4, 8, 12, 32, 70])
+def test_diff_attention_fp32_over_many_keys_of_few_rows(ops, d, rows):
+    """The root mean square error of fp32 over 6000 keys, most sequences' by one workgroup alone.  One rounding of at most half a step at the sum's size for 32 keys, going either way:
+    sqrt(n / 32) of them in a sum, in the values' and in the weights' one: sqrt(2); lambda is 0, so that nothing cancels."""
+    n, units = 6000, 1100
+    q, k = randn(1, 1, rows, 1, 2 * d), randn(2, 1, n, 1, 2 * d)
+    v = randn(3, 1, n, 1, 2 * d) + 1
+    got = ops.diff_attention(*(x.expand(units, -1, -1, -1) for x in (q, k, v)), torch.zeros(4, d, device="cuda"), lambda_init=0.0)
+    p = torch.softmax(q[0, :, 0, :d].double() @ k[0, :, 0, :d].double().t().contiguous() / math.sqrt(d), -1)
+    ref = p @ v[0, :, 0].double()
+    # every sequence, whole or (the last ones) in pieces
+    assert float((got[:, :, 0].double() - ref).flatten(1).norm(dim=1).max() / ref.norm()) <= math.sqrt(2) * math.sqrt(n / 32) * E
