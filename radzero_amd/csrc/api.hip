@@ -1701,9 +1701,10 @@ static const char* diff_attention_error(const rz_diff_attention_args* a) {
     if (!(a->scale > 0.f) || a->scale > 1e30f) return "rz_diff_attention: scale must be positive and finite";
     if (a->norm_weight_dev && !(a->norm_eps >= 0.f)) return "rz_diff_attention: norm_eps must not be negative";
     // 32-bit row numbers and grids inside; offsets are 64-bit
-    if (a->n_k > (1 << 30) || (int64_t)a->n_q * a->heads > (1 << 30) || (int64_t)a->batch * a->heads * a->n_q > INT32_MAX ||
-        (int64_t)a->batch * a->kv_heads * ((int64_t)a->n_q * (a->heads / a->kv_heads) / 64 + 1) > (1 << 23))         // workgroups: a launch takes less than 2^32 threads
-        return "rz_diff_attention: too many rows";
+    if (a->n_k > (1 << 30) || (int64_t)a->n_q * a->heads > (1 << 30) || (int64_t)a->batch * a->heads * a->n_q > INT32_MAX) return "rz_diff_attention: too many rows";
+    // a launch takes less than 2^32 threads: blocks of 64 rows at most 2^23, and a form of smaller blocks (a handful of rows) less than 2^24 workgroups of 256
+    const int64_t blocks = (int64_t)a->batch * a->kv_heads * ((int64_t)a->n_q * (a->heads / a->kv_heads) / 64 + 1);
+    if (blocks > (1 << 23) || (blocks > (1 << 22) && a->batch && a->n_q && diff_attention_workgroups(*a) >= (1 << 24))) return "rz_diff_attention: too many rows";
     return nullptr;
 }
 

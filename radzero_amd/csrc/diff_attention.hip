@@ -1374,6 +1374,8 @@ template <typename T, int D, bool KEYS, typename F> Args make(const rz_diff_atte
     return x;
 }
 
+int groups(const Args& x) { return x.shared ? x.slots : x.full + x.ranges; }
+
 template <typename T, int D, bool KEYS, typename F> hipError_t launch(void (*k)(Args), const rz_diff_attention_args& a, void* ws, hipStream_t s) {
     const Args x = make<T, D, KEYS, F>(a, ws);
     if (F::kLds > 64 * 1024) {
@@ -1386,7 +1388,7 @@ template <typename T, int D, bool KEYS, typename F> hipError_t launch(void (*k)(
         }
     }
     const int tail = x.units - x.full;
-    hipLaunchKernelGGL(k, dim3((unsigned)(x.shared ? x.slots : x.full + x.ranges)), dim3(64 * F::W), F::kLds, s, x);
+    hipLaunchKernelGGL(k, dim3((unsigned)groups(x)), dim3(64 * F::W), F::kLds, s, x);
     if (hipError_t err = hipGetLastError(); err != hipSuccess || !tail) return err;
     hipLaunchKernelGGL((diff_attention_join_kernel<T, D>), dim3((unsigned)(((int64_t)tail * x.part_rows + 3) / 4)), dim3(256), 0, s, x, F::BR);
     return hipGetLastError();
@@ -1407,11 +1409,17 @@ template <typename T, int D, typename Use> auto with_form(const rz_diff_attentio
 template <typename T, int D> size_t workspace(const rz_diff_attention_args& a) {
     return with_form<T, D>(a, [&](auto keys, auto form, auto) { return (size_t)parts(make<T, D, decltype(keys)::value, decltype(form)>(a, nullptr)) * (4 * D + 4) * sizeof(float); });
 }
+template <typename T, int D> int workgroups(const rz_diff_attention_args& a) {
+    return with_form<T, D>(a, [&](auto keys, auto form, auto) { return groups(make<T, D, decltype(keys)::value, decltype(form)>(a, nullptr)); });
+}
 template <typename T, int D> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
     return with_form<T, D>(a, [&](auto keys, auto form, auto kernel) { return launch<T, D, decltype(keys)::value, decltype(form)>(kernel, a, ws, s); });
 }
 template <typename T> size_t workspace(const rz_diff_attention_args& a) {
     return a.head_dim == 32 ? workspace<T, 32>(a) : a.head_dim == 64 ? workspace<T, 64>(a) : workspace<T, 128>(a);
+}
+template <typename T> int workgroups(const rz_diff_attention_args& a) {
+    return a.head_dim == 32 ? workgroups<T, 32>(a) : a.head_dim == 64 ? workgroups<T, 64>(a) : workgroups<T, 128>(a);
 }
 template <typename T> hipError_t launch(const rz_diff_attention_args& a, void* ws, hipStream_t s) {
     return a.head_dim == 32 ? launch<T, 32>(a, ws, s) : a.head_dim == 64 ? launch<T, 64>(a, ws, s) : launch<T, 128>(a, ws, s);
@@ -1421,6 +1429,10 @@ template <typename T> hipError_t launch(const rz_diff_attention_args& a, void* w
 
 size_t diff_attention_workspace_bytes(const rz_diff_attention_args& a) {
     return a.dtype == DT_F32 ? workspace<float>(a) : a.dtype == DT_BF16 ? workspace<bf16_t>(a) : workspace<f16_t>(a);
+}
+
+int diff_attention_workgroups(const rz_diff_attention_args& a) {
+    return a.dtype == DT_F32 ? workgroups<float>(a) : a.dtype == DT_BF16 ? workgroups<bf16_t>(a) : workgroups<f16_t>(a);
 }
 
 hipError_t launch_diff_attention(const rz_diff_attention_args& a, void* ws, hipStream_t s) {

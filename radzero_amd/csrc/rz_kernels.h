@@ -186,6 +186,7 @@ hipError_t launch_preprocess_batch(const void* descs_host, int n, int max_ph, in
 // operators of a differential-attention block; arguments as the C-ABI takes them, checked by api.hip
 hipError_t launch_rotary(const rz_rotary_args& a, hipStream_t s);
 size_t diff_attention_workspace_bytes(const rz_diff_attention_args& a);
+int diff_attention_workgroups(const rz_diff_attention_args& a);
 hipError_t launch_diff_attention(const rz_diff_attention_args& a, void* ws, hipStream_t s);
 hipError_t launch_residual_norm(const rz_residual_norm_args& a, hipStream_t s);
 

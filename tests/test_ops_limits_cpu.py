@@ -1,0 +1,22 @@
+"""radzero_amd.ops and the operators' C entries at the ends of what they take, without a GPU."""
+import ctypes
+
+import pytest
+
+from radzero_amd import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("n_q", [5, 8])
+def test_diff_attention_counts_the_workgroups_of_the_form_it_takes(lib, head_dim, n_q):
+    """fp32 takes five to eight rows as two blocks: 2^23 sequences' key heads would be 2^24 workgroups of 256 threads, one more than a launch takes."""
+    a = _lib.RzDiffAttentionArgs(dtype=0, batch=1 << 22, heads=2, kv_heads=2, n_q=n_q, n_k=5, head_dim=head_dim, causal=0, scale=0.125, lambda_init=0.2, out_scale=1.0, q_dev=16,
+                                 k_dev=32, v_dev=48, out_dev=64, lambda_qk_dev=16)
+    assert lib.rz_diff_attention(ctypes.byref(a), 16, 1 << 40, None) == 10001
+    assert b"too many rows" in lib.rz_last_error()
+    assert lib.rz_diff_attention_workspace(ctypes.byref(a)) == 0

@@ -332,6 +332,7 @@ hipError_t launch_rotary(const rz_rotary_args& a, hipStream_t) {
     return hipSuccess;
 }
 size_t diff_attention_workspace_bytes(const rz_diff_attention_args& a) { return a.n_k > 4096 ? (size_t)a.batch * a.heads * a.n_q * 16 : 0; }
+int diff_attention_workgroups(const rz_diff_attention_args&) { return 1; }
 hipError_t launch_diff_attention(const rz_diff_attention_args& a, void* ws, hipStream_t) {
     const size_t es = esz(a.dtype), cols = 2 * (size_t)a.head_dim;
     rows3((void*)a.q_dev, a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.batch, a.n_q, a.heads, cols, es, false, "diff_attention q");
