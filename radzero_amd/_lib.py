@@ -34,6 +34,13 @@ ARCH = "gfx950"
 # no packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): hipcc -O3 makes it from ordinary float code, and on these machines some of its
 # forms have given wrong results now and then, without an error.  (hipcc's host pass warns that it does not know the feature: harmless.)
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+LINK_FLAGS = [f"--offload-arch={ARCH}", "-shared", "-fPIC"]
+
+
+def _flags() -> list:
+    """What every source is compiled with, but for its include folders."""
+    return [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Werror=uninitialized", "-Werror=return-type", *NO_PACKED_F32,
+            *(["-DRZ_EXPERIMENTS"] if EXPERIMENTS else []), *os.environ.get("RZ_CXXFLAGS", "").split()]      # RZ_CXXFLAGS: A/B builds of a tunable (with RZ_LIB_PATH)
 
 RZ_F32, RZ_BF16, RZ_F16 = 0, 1, 2
 PROF_FAMILIES = ("attn", "gemm", "rowops", "vlcabs", "post")
@@ -55,11 +62,11 @@ STAMP_PATH = LIB_PATH + ".stamp"
 
 
 def _source_digest() -> str:
-    """sha256 over the CONTENTS of every source / header the library is built from (+ the build flavour and extra flags): the rebuild decision must not
+    """sha256 over the CONTENTS of every source / header the library is built from (+ the sources' list and all flags): the rebuild decision must not
     depend on file times — a snapshot copied to another machine (gpurun, the driver's round-end run) keeps contents, not necessarily mtime order."""
     import hashlib
     h = hashlib.sha256()
-    h.update(("experiments" if EXPERIMENTS else "product").encode() + os.environ.get("RZ_CXXFLAGS", "").encode() + " ".join(NO_PACKED_F32).encode())
+    h.update(repr((SOURCES, _flags(), sorted(EXTRA_FLAGS.items()), LINK_FLAGS)).encode())
     for d in sorted(os.path.abspath(p) for p in _all_deps() if os.path.isfile(p)):
         h.update(os.path.basename(d).encode())
         with open(d, "rb") as f:
@@ -107,8 +114,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def _build_locked(obj_dir: str, verbose: bool, force: bool = False) -> str:
-    flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Werror=uninitialized",
-             "-Werror=return-type", *NO_PACKED_F32, f"-I{CSRC}"] + (["-DRZ_EXPERIMENTS", f"-I{EXP_SRC}"] if EXPERIMENTS else []) + os.environ.get("RZ_CXXFLAGS", "").split()   # RZ_CXXFLAGS: A/B builds of a tunable (with RZ_LIB_PATH)
+    flags = [*_flags(), f"-I{CSRC}", *([f"-I{EXP_SRC}"] if EXPERIMENTS else [])]
     tag = f".{os.getpid()}.tmp"
 
     def cc(src):
@@ -130,8 +136,7 @@ def _build_locked(obj_dir: str, verbose: bool, force: bool = False) -> str:
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(cc, SOURCES))
-    r = subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", LIB_PATH + tag, *objs],
-                       capture_output=True, text=True)
+    r = subprocess.run([HIPCC, *LINK_FLAGS, "-o", LIB_PATH + tag, *objs], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(LIB_PATH + tag, LIB_PATH)

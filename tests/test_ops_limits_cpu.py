@@ -20,3 +20,14 @@ def test_diff_attention_counts_the_workgroups_of_the_form_it_takes(lib, head_dim
     assert lib.rz_diff_attention(ctypes.byref(a), 16, 1 << 40, None) == 10001
     assert b"too many rows" in lib.rz_last_error()
     assert lib.rz_diff_attention_workspace(ctypes.byref(a)) == 0
+
+
+@pytest.mark.parametrize("change", [lambda m: m.setitem(_lib.EXTRA_FLAGS, "rotary.hip", ["-g"]), lambda m: m.setitem(_lib.EXTRA_FLAGS, "diff_attention.hip", []),
+                                    lambda m: m.setattr(_lib, "NO_PACKED_F32", []), lambda m: m.setattr(_lib, "ARCH", "gfx942"), lambda m: m.setattr(_lib, "LINK_FLAGS", []),
+                                    lambda m: m.setenv("RZ_CXXFLAGS", "-DX=1"), lambda m: m.setattr(_lib, "SOURCES", _lib.SOURCES[1:])])
+def test_every_flag_asks_for_a_new_library(monkeypatch, change):
+    """A library built with other flags than the tree's is not taken for the tree's, and the same tree elsewhere asks for the same library."""
+    was = _lib._source_digest()
+    assert _lib._source_digest() == was and _lib.CSRC not in " ".join(_lib._flags())
+    change(monkeypatch)
+    assert _lib._source_digest() != was
