@@ -1,5 +1,8 @@
 """radzero_amd.ops and the operators' C entries at the ends of what they take, without a GPU."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -31,3 +34,16 @@ def test_every_flag_asks_for_a_new_library(monkeypatch, change):
     assert _lib._source_digest() == was and _lib.CSRC not in " ".join(_lib._flags())
     change(monkeypatch)
     assert _lib._source_digest() != was
+
+
+def test_variants_are_compiled_as_the_library_is(tmp_path):
+    """tools/build_variant.py leaves out none of the library's flags, the one against packed fp32 arithmetic among them."""
+    _lib.build()                                         # current, so that the compiler below is asked for the variant alone
+    said, compiler = tmp_path / "said", tmp_path / "hipcc"
+    compiler.write_text(f'#!/bin/sh\necho "$@" >> {said}\n')
+    compiler.chmod(0o755)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, os.path.join(root, "tools", "build_variant.py"), "x", "diff_attention.hip", "-DX=1"], check=True, env={**os.environ, "HIPCC": str(compiler)})
+    compiled = said.read_text().splitlines()[0]
+    for flag in [*_lib._flags(), *_lib.EXTRA_FLAGS["diff_attention.hip"], "-DX=1"]:
+        assert flag in compiled.split(), flag

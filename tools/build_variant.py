@@ -9,9 +9,8 @@ name, src, flags = sys.argv[1], sys.argv[2], sys.argv[3:]
 _lib.build()                                             # the product objects are current
 obj_dir = os.path.join(_lib.PKG_DIR, "build")
 vobj = os.path.join(obj_dir, f"variant_{name}_{src.replace('.hip', '.o')}")
-base = [f"--offload-arch={_lib.ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
-subprocess.run([_lib.HIPCC, *base, *_lib.EXTRA_FLAGS.get(src, []), *flags, "-c", os.path.join(_lib.CSRC, src), "-o", vobj], check=True)
+subprocess.run([_lib.HIPCC, *_lib._flags(), f"-I{_lib.CSRC}", *_lib.EXTRA_FLAGS.get(src, []), *flags, "-c", os.path.join(_lib.CSRC, src), "-o", vobj], check=True)
 objs = [vobj if s == src else os.path.join(obj_dir, s.replace(".hip", ".o")) for s in _lib.SOURCES]
 out = os.path.join(_lib.PKG_DIR, f"libradzero_hip_{name}.so")
-subprocess.run([_lib.HIPCC, f"--offload-arch={_lib.ARCH}", "-shared", "-fPIC", "-o", out, *objs], check=True)
+subprocess.run([_lib.HIPCC, *_lib.LINK_FLAGS, "-o", out, *objs], check=True)
 print(out)
