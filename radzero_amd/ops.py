@@ -162,6 +162,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torc
     _need(layout in _LAYOUT, "layout must be half or interleaved")
     _need(isinstance(freqs, torch.Tensor) and freqs.dtype is torch.float64 and freqs.dim() in (1, 2) and freqs.device == dev and freqs.is_contiguous(),
           "freqs must be contiguous float64 (pairs,) or (axes, pairs) on q's device")
+    _need(not (freqs.requires_grad and torch.is_grad_enabled()), "freqs asks for a gradient: these operators are forward only (torch.no_grad())")
     pos = positions
     _need(isinstance(pos, torch.Tensor) and pos.dtype is torch.int64 and pos.device == dev, "positions must be int64 on q's device")
     shape, strides, axes = tuple(pos.shape), pos.stride(), 1

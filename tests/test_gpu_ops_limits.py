@@ -107,3 +107,38 @@ def test_diff_attention_fp32_over_many_keys_of_few_rows(ops, d, rows):
     ref = p @ v[0, :, 0].double()
     # every sequence, whole or (the last ones) in pieces
     assert float((got[:, :, 0].double() - ref).flatten(1).norm(dim=1).max() / ref.norm()) <= math.sqrt(2) * math.sqrt(n / 32) * E
+
+
+def block_calls(ops):
+    """{operator: (call with a dict of changed arguments, its arguments)}, small."""
+    h = randn(11, 2, 4, 64)
+    args = {
+        "rotary": dict(q=randn(1, 2, 4, 2, 64), k=randn(2, 2, 4, 2, 64), positions=torch.arange(4, device="cuda"), freqs=ops.rotary_frequencies(64, device="cuda")[0]),
+        "diff_attention": dict(q=randn(3, 2, 4, 2, 64), k=randn(4, 2, 5, 2, 64), v=randn(5, 2, 5, 2, 64), lambda_qk=randn(6, 4, 32), lambda_init=0.3, norm_weight=randn(7, 64)),
+        "residual_norm": dict(residual=h, y=randn(8, 2, 4, 64), pre_norm=ops.Norm(randn(9, 64), randn(10, 64)), post_norm=ops.Norm(randn(12, 64), randn(13, 64)), scale=randn(14, 64),
+                              gate=randn(15, 2, 64)),
+    }
+    return {name: (lambda name=name, **change: getattr(ops, name)(**{**args[name], **change}), args[name]) for name in args}
+
+
+INPUTS = [("rotary", n) for n in ("q", "k", "freqs")] + [("diff_attention", n) for n in ("q", "k", "v", "lambda_qk", "norm_weight")] + [
+    ("residual_norm", n) for n in ("residual", "y", "scale", "gate", "pre_norm.weight", "pre_norm.bias", "post_norm.weight", "post_norm.bias")]
+
+
+def changed(args, name, f):
+    """{argument: itself with f applied to the tensor `name`}."""
+    name, _, part = name.partition(".")
+    return {name: args[name]._replace(**{part: f(getattr(args[name], part))}) if part else f(args[name])}
+
+
+@pytest.mark.parametrize("operator,name", INPUTS, ids=lambda x: x)
+def test_operators_refuse_every_input_that_asks_for_a_gradient(ops, operator, name):
+    call, args = block_calls(ops)[operator]
+    want = call()
+    asking = changed(args, name, lambda t: t.clone().requires_grad_())
+    with pytest.raises(ValueError, match="gradient"):
+        call(**asking)
+    with torch.no_grad():
+        got = call(**asking)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
