@@ -2,7 +2,7 @@
 block with its gate and residual scale (rz_rotary, rz_diff_attention, rz_residual_norm of include/radzero_hip.h).
 
 They work on GPU tensors alone, on the current stream of the tensors' device, never wait for it and may be captured into a graph.  They are
-forward only, like everything here: an input that asks for a gradient is refused.  Types are float32, bfloat16 and float16 for tokens;
+forward only, like everything here: an input that asks for a gradient, or carries a forward-mode one, is refused.  Types are float32, bfloat16 and float16 for tokens;
 weights, gates and lambda vectors are float32.  Strides are free except that columns are contiguous; what a kernel cannot take raises ValueError.
 
     freqs, amplitude = rotary_frequencies(64, axes=2, device="cuda")
@@ -17,6 +17,7 @@ import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -60,6 +61,17 @@ def _vector(x, name, shape, device):
         _need(x.device == device and x.is_contiguous(), f"{name} must be contiguous on {device}")
         _need(not torch.is_grad_enabled(), f"{name} asks for a gradient: these operators are forward only (torch.no_grad())")
     return x.data_ptr()
+
+
+def _no_tangents(*inputs):
+    """Tensors that carry a forward-mode derivative do not say so in requires_grad."""
+    for x in inputs:
+        _need(not isinstance(x, torch.Tensor) or forward_ad.unpack_dual(x).tangent is None, "an input carries a forward-mode derivative: these operators have none")
+
+
+def _differentiating():
+    """Inside a level of forward-mode differentiation (then inputs are looked at one by one)?"""
+    return getattr(forward_ad, "_current_level", 0) >= 0
 
 
 _empty_like = torch.empty_like
@@ -149,6 +161,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torc
     positions: int64, (tokens,) or (batch, tokens), with a last dimension of `axes` if freqs has two dimensions; |position| < 2^31.
     layout: "half" pairs column p with p + rotary_dim / 2, "interleaved" 2 p with 2 p + 1.
     out: tensors to write (q_out, or (q_out, k_out)); the inputs themselves are fine.  Returns q_out, or (q_out, k_out) with k."""
+    if _differentiating():
+        _no_tangents(q, k, freqs)
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES and q.dim() == 4 and q.stride(3) == 1 and not q.requires_grad):
         _tokens(q, "q", 4)
     b, n, hq, d = q.shape
@@ -201,6 +215,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
     a row's sum together, over up to 2^22 keys); float32 products may be taken from three bf16 parts of each
     operand (2^-22 of |a||b| off; an infinity that a query sees then gives NaN).
     16-byte alignment of q, k, v and out and of their strides is required.  Returns (batch, n_q, heads, 2 d), in `out` (no input's memory) if given."""
+    if _differentiating():
+        _no_tangents(q, k, v, lambda_qk, norm_weight)
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES and q.dim() == 4 and not q.requires_grad):
         _tokens(q, "q", 4)
     dev, dt = q.device, q.dtype
@@ -256,6 +272,8 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
     gate float32: (dim,), (batch, dim), (batch, rows, dim) or, for a residual of two dimensions, (dim,) or (rows, dim).
     x has y's type (without y: `dtype`, else the residual's).  pre_norm None: x is None.  out: (r, x) to write; r may be `residual`, x may be `y`.
     pre_norm's statistics are those of r in float32, before it is rounded to the residual's type."""
+    if _differentiating():
+        _no_tangents(residual, y, scale, gate, *(pre_norm or ()), *(post_norm or ()))
     nd = residual.dim() if isinstance(residual, torch.Tensor) else 0
     _need(nd == 2 or nd == 3, "residual must be (rows, dim) or (batch, rows, dim)")
     hs = residual.stride()

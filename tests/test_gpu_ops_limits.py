@@ -142,3 +142,15 @@ def test_operators_refuse_every_input_that_asks_for_a_gradient(ops, operator, na
         got = call(**asking)
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("operator,name", INPUTS, ids=lambda x: x)
+def test_operators_refuse_every_input_with_a_forward_derivative(ops, operator, name):
+    call, args = block_calls(ops)[operator]
+    want = call()
+    with torch.autograd.forward_ad.dual_level():
+        for x, y in zip(call(), want):                   # plain inputs inside such a level
+            assert torch.equal(x, y)
+        dual = changed(args, name, lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(ValueError, match="forward-mode"):
+            call(**dual)
