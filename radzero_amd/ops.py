@@ -18,6 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -86,7 +87,17 @@ def _output(out, like_shape, dtype, device, name):
     _need(isinstance(out, torch.Tensor) and out.shape == like_shape and out.dtype == dtype and out.device == device,
           f"{name} must be {dtype} {tuple(like_shape)} on {device}")
     _need(all(s for s, n in zip(out.stride(), out.shape) if n > 1) and (out.stride(-1) == 1 or out.shape[-1] == 1), f"{name}: columns must be contiguous, rows apart")
+    _need(not (out.requires_grad and torch.is_grad_enabled()), f"{name} asks for a gradient: these operators are forward only (torch.no_grad())")
+    if _differentiating():
+        _no_tangents(out)
     return out
+
+
+def _written(*outs):
+    """Tensors of the caller's were written: a backward pass that saved one of them before has to notice, as after any in-place operation."""
+    for x in outs:
+        if x is not None:
+            increment_version(x)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -198,6 +209,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torc
     _call("rz_rotary", _STREAM, dev, _lib.RzRotaryArgs.pack(
         _DTYPES[dt], _LAYOUT[layout], b, n, hq, hk, d, 2 * freqs.numel(), axes, amplitude, q.data_ptr(), qs[0], qs[1], qs[2], kp, ks[0], ks[1], ks[2],
         qo.data_ptr(), qos[0], qos[1], qos[2], kop, kos[0], kos[1], kos[2], pos.data_ptr(), strides[0] if len(shape) == 2 else 0, strides[-1], freqs.data_ptr()))
+    if out is not None:
+        _written(qo, ko)
     return qo if k is None else (qo, ko)
 
 
@@ -251,7 +264,7 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
         if n_k > 1 and x.stride(1) != 1:
             x = x.contiguous()
         attention_mask, mask, mask_stride = x, x.data_ptr(), x.stride(0)
-    out = _new(q) if out is None else _output(out, q.shape, dt, dev, "out")
+    given, out = out, _new(q) if out is None else _output(out, q.shape, dt, dev, "out")
     os = out.stride()
     args = _lib.RzDiffAttentionArgs.pack(
         _DTYPES[dt], b, h, hk, n_q, n_k, d, _CAUSAL[causal], d ** -0.5 if scale is None else scale, lambda_init, norm_eps, out_scale,
@@ -260,6 +273,7 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
     need = _fn("rz_diff_attention_workspace")(args)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _call("rz_diff_attention", _WORKSPACE_STREAM, dev, args, ws.data_ptr() if need else 0, need)
+    _written(given)
     return out
 
 
@@ -328,4 +342,6 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
     _call("rz_residual_norm", _STREAM, dev, _lib.RzResidualNormArgs.pack(
         _DTYPES[t], _DTYPES[rt], batch, rows, dim, post_kind, pre_kind, alpha, post_eps, pre_eps, yp, ys[0], ys[1], residual.data_ptr(), hs[0], hs[1], rp, rs[0], rs[1],
         xp, xs[0], xs[1], post_w, post_b, _vector(scale, "scale", (dim,), dev), gp, gb, gr, pre_w, pre_b))
+    if out is not None:
+        _written(*out)
     return ro, xo

@@ -154,3 +154,33 @@ def test_operators_refuse_every_input_with_a_forward_derivative(ops, operator, n
         dual = changed(args, name, lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
         with pytest.raises(ValueError, match="forward-mode"):
             call(**dual)
+
+
+OUTPUTS = [("rotary", lambda a: ("q", "k")), ("diff_attention", lambda a: ("q",)), ("residual_norm", lambda a: ("residual", "y"))]
+
+
+@pytest.mark.parametrize("operator,like", OUTPUTS, ids=lambda x: x if isinstance(x, str) else "")
+def test_outputs_count_as_written_in_place(ops, operator, like):
+    """A backward pass that saved a tensor before an operator wrote it raises, as it does for any in-place operation, also without grad mode; an output that asks for a gradient or
+    carries a forward-mode one is refused."""
+    call, args = block_calls(ops)[operator]
+    given = lambda outs: outs[0] if operator == "diff_attention" else tuple(outs)      # noqa: E731
+    names = like(args)
+    for i in range(len(names)):
+        outs = [torch.zeros_like(args[n]) for n in names]
+        w = torch.ones((), device="cuda", requires_grad=True)
+        loss = (outs[i] * w).sum()
+        with torch.no_grad():
+            got = call(out=given(outs))
+        assert all(x is y for x, y in zip(outs, got if isinstance(got, tuple) else (got,)))
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+        outs[i] = outs[i].detach().requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            call(out=given(outs))
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+            outs[i] = torch.autograd.forward_ad.make_dual(torch.zeros_like(args[names[i]]), torch.ones_like(args[names[i]]))
+            call(out=given(outs))
+    with torch.inference_mode():
+        outs = [torch.zeros_like(args[n]) for n in names]
+        call(out=given(outs))
