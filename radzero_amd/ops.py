@@ -285,6 +285,7 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
     residual (rows, dim) or (batch, rows, dim), float32 or y's type; y of the same shape (None: r = alpha * residual).  scale float32 (dim,).
     gate float32: (dim,), (batch, dim), (batch, rows, dim) or, for a residual of two dimensions, (dim,) or (rows, dim).
     x has y's type (without y: `dtype`, else the residual's).  pre_norm None: x is None.  out: (r, x) to write; r may be `residual`, x may be `y`.
+    Without y and alpha, and no place given for it, r is `residual` itself (a copy if x is written over that).
     pre_norm's statistics are those of r in float32, before it is rounded to the residual's type."""
     if _differentiating():
         _no_tangents(residual, y, scale, gate, *(pre_norm or ()), *(post_norm or ()))
@@ -317,7 +318,7 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
         gb, gr = (0, 0) if gate.dim() == 1 else (st[0], st[1]) if gate.dim() == 3 else (st[0], 0) if nd == 3 else (0, st[0])
     ro, xo = (None, None) if out is None else out
     rp, rs, xp, xs = 0, (0, 0, 0), 0, (0, 0, 0)
-    if y is not None or alpha != 1.0 or ro is not None or pre_norm is None:
+    if y is not None or alpha != 1.0 or ro is not None or pre_norm is None or (xo is not None and xo.data_ptr() == residual.data_ptr()):      # x over the residual: r is a copy
         ro = _new(residual) if ro is None else _output(ro, shape, rt, dev, "out[0]")
         rp, rs = ro.data_ptr(), ro.stride()
     else:

@@ -184,3 +184,12 @@ def test_outputs_count_as_written_in_place(ops, operator, like):
     with torch.inference_mode():
         outs = [torch.zeros_like(args[n]) for n in names]
         call(out=given(outs))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_residual_norm_over_its_residual_keeps_the_residual(ops, dtype):
+    """x written where the residual stands, with nothing added to it: r still is the residual."""
+    h = randn(21, 3, 5, 100, dtype=dtype)
+    was, want = h.clone(), ops.residual_norm(h, pre_norm=ops.Norm())[1]
+    r, x = ops.residual_norm(h, pre_norm=ops.Norm(), out=(None, h))
+    assert x is h and torch.equal(x, want) and torch.equal(r, was)
