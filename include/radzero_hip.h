@@ -239,7 +239,7 @@ int rz_patch_embed(int dtype, const float* pixel_values_dev, int batch, int chan
  *   columns from rotary_dim (even, <= head_dim <= 1024) on pass through.  k_heads = 0: q alone.
  *   positions_dev int64, axis x of token n of batch entry b at [b * positions_batch_stride + n * positions_token_stride + x] (any sign, |position| < 2^31;
  *   a batch stride of 0 shares them); freqs_dev double (rotary_dim / 2): radians per position, pairs dealt to the n_axes axes in equal runs.
- *   Outputs may be the inputs themselves (in place, same strides); they may not overlap them otherwise. */
+ *   An output may be its input itself (in place, same strides); what overlaps otherwise is refused. */
 enum rz_rotary_layout { RZ_ROTARY_HALF = 0, RZ_ROTARY_INTERLEAVED = 1 };
 typedef struct rz_rotary_args {
     int32_t dtype, layout, batch, tokens, q_heads, k_heads, head_dim, rotary_dim, n_axes;
@@ -286,8 +286,8 @@ int rz_diff_attention(const rz_diff_attention_args* args, void* workspace_dev, s
 
 /* The norms either side of a block with its gate and residual scale: t = post_norm(y); r = alpha * resid + scale * gate * t -> resid_out;
  *   pre_norm(r) -> out (the next block's operand).  y_dev, out_dev `dtype`; resid `resid_dtype` (RZ_F32 or `dtype`); everything else fp32.
- *   y_dev NULL: r = alpha * resid.  resid_out_dev / out_dev NULL: not written (not both); resid_out_dev may be resid_dev, out_dev may be y_dev or, of
- *   one type, resid_dev (same strides).  Norm kinds: RZ_NORM_NONE, RZ_NORM_LAYER, RZ_NORM_RMS; weights and biases (dim) or NULL; scale_dev (dim) or NULL;
+ *   y_dev NULL: r = alpha * resid.  resid_out_dev / out_dev NULL: not written (not both); either may be resid_dev or y_dev itself (same type and strides), what
+ *   overlaps otherwise is refused.  Norm kinds: RZ_NORM_NONE, RZ_NORM_LAYER, RZ_NORM_RMS; weights and biases (dim) or NULL; scale_dev (dim) or NULL;
  *   gate_dev row of batch entry b, row n at b * gate_batch_stride + n * gate_row_stride (0 = shared), or NULL.  1 <= dim <= 16384, any alignment.
  *   The statistics of pre_norm are those of r in fp32, before it is rounded to resid_dtype. */
 enum rz_norm_kind { RZ_NORM_NONE = 0, RZ_NORM_LAYER = 1, RZ_NORM_RMS = 2 };

@@ -1674,6 +1674,56 @@ int rz_patch_embed(int dtype, const float* px, int B, int C, int Himg, int Wimg,
     return 0;
 }
 
+// Rows of an operator's tensor: `cols` contiguous elements of `size` bytes at every step of three strides (elements).
+struct Rows {
+    const void* p;
+    int64_t n[3], stride[3], cols, size;
+    bool same(const Rows& o) const {                      // the same elements in the same places
+        for (int i = 0; i < 3; ++i)
+            if (n[i] != o.n[i] || (n[i] > 1 && stride[i] != o.stride[i])) return false;
+        return p == o.p && cols == o.cols && size == o.size;
+    }
+};
+
+// Whether two of them share an element.  A row of a begins D + (sum of e_i stride_i) bytes behind one of b, e_i over a range for every stride of either: the largest strides
+// first, only those e_i from which the rest can still bring the two rows together (hardly ever more than two).  Given up, as apart, after 100000 steps.
+struct Meeting {
+    __int128 stride[6], low[6], high[6], rest_low[7], rest_high[7], row_a, row_b;
+    int terms = 0, steps = 0;
+    bool from(__int128 at, int k) {
+        if (++steps > 100000 || at + rest_low[k] >= row_b || at + rest_high[k] <= -row_a) return false;
+        if (k == terms) return true;
+        const auto down = [](__int128 x, __int128 y) { return x / y - (x % y != 0 && (x < 0) != (y < 0)); };
+        const __int128 first = down(-row_a - at - rest_high[k + 1], stride[k]) + 1, last = -down(at + rest_low[k + 1] - row_b, stride[k]) - 1;
+        for (__int128 e = first > low[k] ? first : low[k]; e <= (last < high[k] ? last : high[k]) && steps <= 100000; ++e)
+            if (from(at + e * stride[k], k + 1)) return true;
+        return false;
+    }
+};
+static bool overlap(const Rows& a, const Rows& b) {
+    Meeting m;
+    m.row_a = a.cols * a.size, m.row_b = b.cols * b.size;
+    for (int t = 0; t < 6; ++t) {
+        const Rows& x = t < 3 ? a : b;
+        const int64_t n = x.n[t % 3];
+        if (n <= 0) return false;
+        __int128 s = (__int128)x.stride[t % 3] * x.size, low = t < 3 ? 0 : 1 - n, high = t < 3 ? n - 1 : 0;
+        if (s < 0) s = -s, std::swap(low, high), low = -low, high = -high;
+        if (n == 1 || s == 0) continue;
+        int at = 0;
+        while (at < m.terms && m.stride[at] > s) ++at;
+        if (at < m.terms && m.stride[at] == s) {
+            m.low[at] += low, m.high[at] += high;
+            continue;
+        }
+        for (int i = m.terms++; i > at; --i) m.stride[i] = m.stride[i - 1], m.low[i] = m.low[i - 1], m.high[i] = m.high[i - 1];
+        m.stride[at] = s, m.low[at] = low, m.high[at] = high;
+    }
+    m.rest_low[m.terms] = m.rest_high[m.terms] = 0;
+    for (int i = m.terms - 1; i >= 0; --i) m.rest_low[i] = m.rest_low[i + 1] + m.low[i] * m.stride[i], m.rest_high[i] = m.rest_high[i + 1] + m.high[i] * m.stride[i];
+    return m.from((__int128)(intptr_t)a.p - (__int128)(intptr_t)b.p, 0);
+}
+
 int rz_rotary(const rz_rotary_args* a, void* stream) {
     if (!a) return fail(RZ_ERR_INVALID, "rz_rotary: null argument");
     if (a->dtype < 0 || a->dtype > 2) return fail(RZ_ERR_INVALID, "rz_rotary: dtype");
@@ -1685,8 +1735,15 @@ int rz_rotary(const rz_rotary_args* a, void* stream) {
     if (a->n_axes < 1 || (a->rotary_dim / 2) % a->n_axes) return fail(RZ_ERR_INVALID, "rz_rotary: the rotary pairs must be a multiple of the axes");
     if (a->batch == 0 || a->tokens == 0) return 0;
     if ((int64_t)a->batch * a->tokens > INT32_MAX) return fail(RZ_ERR_INVALID, "rz_rotary: too many tokens");
-    if (!a->q_dev || !a->q_out_dev || (a->k_heads && (!a->k_dev || !a->k_out_dev)) || !a->positions_dev || !a->freqs_dev)
-        return fail(RZ_ERR_INVALID, "rz_rotary: null pointer");
+    if (!a->q_dev || !a->q_out_dev || (a->k_heads && (!a->k_dev || !a->k_out_dev))) return fail(RZ_ERR_INVALID, "rz_rotary: null pointer");
+    const int64_t size = a->dtype == RZ_F32 ? 4 : 2;
+    const Rows q{a->q_dev, {a->batch, a->tokens, a->q_heads}, {a->q_batch_stride, a->q_token_stride, a->q_head_stride}, a->head_dim, size};
+    const Rows qo{a->q_out_dev, {a->batch, a->tokens, a->q_heads}, {a->q_out_batch_stride, a->q_out_token_stride, a->q_out_head_stride}, a->head_dim, size};
+    const Rows k{a->k_dev, {a->batch, a->tokens, a->k_heads}, {a->k_batch_stride, a->k_token_stride, a->k_head_stride}, a->head_dim, size};
+    const Rows ko{a->k_out_dev, {a->batch, a->tokens, a->k_heads}, {a->k_out_batch_stride, a->k_out_token_stride, a->k_out_head_stride}, a->head_dim, size};
+    if ((!qo.same(q) && overlap(qo, q)) || (!ko.same(k) && overlap(ko, k)) || overlap(qo, k) || overlap(ko, q) || overlap(qo, ko))
+        return fail(RZ_ERR_INVALID, "rz_rotary: an output overlaps an input that it is not, or the other output");
+    if (!a->positions_dev || !a->freqs_dev) return fail(RZ_ERR_INVALID, "rz_rotary: null pointer");
     RZ_HIP(launch_rotary(*a, (hipStream_t)stream));
     return 0;
 }
@@ -1721,7 +1778,12 @@ int rz_diff_attention(const rz_diff_attention_args* a, void* workspace, size_t w
         return fail(RZ_ERR_INVALID, "rz_diff_attention: q, k, v, out and their strides must be multiples of 16 bytes");
     const size_t need = diff_attention_workspace_bytes(*a);
     if (need && (!workspace || workspace_bytes < need)) return fail(RZ_ERR_STATE, "rz_diff_attention: workspace too small (rz_diff_attention_workspace)");
-    if (a->out_dev == a->q_dev || (a->n_k && (a->out_dev == a->k_dev || a->out_dev == a->v_dev))) return fail(RZ_ERR_INVALID, "rz_diff_attention: out must not be q, k or v");
+    const int64_t size = a->dtype == RZ_F32 ? 4 : 2, cols = 2 * a->head_dim;
+    const Rows out{a->out_dev, {a->batch, a->n_q, a->heads}, {a->out_batch_stride, a->out_token_stride, a->out_head_stride}, cols, size};
+    if (overlap(out, {a->q_dev, {a->batch, a->n_q, a->heads}, {a->q_batch_stride, a->q_token_stride, a->q_head_stride}, cols, size}) ||
+        overlap(out, {a->k_dev, {a->batch, a->n_k, a->kv_heads}, {a->k_batch_stride, a->k_token_stride, a->k_head_stride}, cols, size}) ||
+        overlap(out, {a->v_dev, {a->batch, a->n_k, a->kv_heads}, {a->v_batch_stride, a->v_token_stride, a->v_head_stride}, cols, size}))
+        return fail(RZ_ERR_INVALID, "rz_diff_attention: out must not be q, k or v, or overlap them");
     RZ_HIP(launch_diff_attention(*a, workspace, (hipStream_t)stream));
     return 0;
 }
@@ -1737,6 +1799,17 @@ int rz_residual_norm(const rz_residual_norm_args* a, void* stream) {
     if (!(a->post_eps >= 0.f) || !(a->pre_eps >= 0.f)) return fail(RZ_ERR_INVALID, "rz_residual_norm: eps must not be negative");
     if (a->batch == 0 || a->rows == 0) return 0;
     if (!a->resid_dev || (!a->resid_out_dev && !a->out_dev)) return fail(RZ_ERR_INVALID, "rz_residual_norm: null pointer");
+    {
+        const int64_t size = a->dtype == RZ_F32 ? 4 : 2, resid_size = a->resid_dtype == RZ_F32 ? 4 : 2, one = 1;
+        const Rows y{a->y_dev, {a->y_dev ? a->batch : 0, a->rows, one}, {a->y_batch_stride, a->y_row_stride, 0}, a->dim, size};
+        const Rows r{a->resid_dev, {a->batch, a->rows, one}, {a->resid_batch_stride, a->resid_row_stride, 0}, a->dim, resid_size};
+        const Rows ro{a->resid_out_dev, {a->resid_out_dev ? a->batch : 0, a->rows, one}, {a->resid_out_batch_stride, a->resid_out_row_stride, 0}, a->dim, resid_size};
+        const Rows xo{a->out_dev, {a->out_dev ? a->batch : 0, a->rows, one}, {a->out_batch_stride, a->out_row_stride, 0}, a->dim, size};
+        for (const Rows& o : {ro, xo})
+            for (const Rows& i : {r, y})
+                if (!o.same(i) && overlap(o, i)) return fail(RZ_ERR_INVALID, "rz_residual_norm: an output overlaps an input that it is not");
+        if (overlap(ro, xo)) return fail(RZ_ERR_INVALID, "rz_residual_norm: the outputs overlap");
+    }
     if (!a->y_dev && (a->post_kind || a->scale_dev || a->gate_dev)) return fail(RZ_ERR_INVALID, "rz_residual_norm: post norm, scale and gate need y");
     if ((int64_t)a->batch * a->rows > INT32_MAX) return fail(RZ_ERR_INVALID, "rz_residual_norm: too many rows");
     RZ_HIP(launch_residual_norm(*a, (hipStream_t)stream));

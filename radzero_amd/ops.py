@@ -171,7 +171,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torc
     freqs: float64, (P,) or (axes, P) as `rotary_frequencies` makes them; the first 2 * freqs.numel() columns turn, the others pass through.
     positions: int64, (tokens,) or (batch, tokens), with a last dimension of `axes` if freqs has two dimensions; |position| < 2^31.
     layout: "half" pairs column p with p + rotary_dim / 2, "interleaved" 2 p with 2 p + 1.
-    out: tensors to write (q_out, or (q_out, k_out)); the inputs themselves are fine.  Returns q_out, or (q_out, k_out) with k."""
+    out: tensors to write (q_out, or (q_out, k_out)); q_out may be q itself, k_out k; no other overlap.  Returns q_out, or (q_out, k_out) with k."""
     if _differentiating():
         _no_tangents(q, k, freqs)
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _DTYPES and q.dim() == 4 and q.stride(3) == 1 and not q.requires_grad):
@@ -284,7 +284,8 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
 
     residual (rows, dim) or (batch, rows, dim), float32 or y's type; y of the same shape (None: r = alpha * residual).  scale float32 (dim,).
     gate float32: (dim,), (batch, dim), (batch, rows, dim) or, for a residual of two dimensions, (dim,) or (rows, dim).
-    x has y's type (without y: `dtype`, else the residual's).  pre_norm None: x is None.  out: (r, x) to write; r may be `residual`, x may be `y`.
+    x has y's type (without y: `dtype`, else the residual's).  pre_norm None: x is None.  out: (r, x) to write; either may be `residual` or `y` itself,
+    no other overlap.
     Without y and alpha, and no place given for it, r is `residual` itself (a copy if x is written over that).
     pre_norm's statistics are those of r in float32, before it is rounded to the residual's type."""
     if _differentiating():

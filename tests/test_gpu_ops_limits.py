@@ -193,3 +193,31 @@ def test_residual_norm_over_its_residual_keeps_the_residual(ops, dtype):
     was, want = h.clone(), ops.residual_norm(h, pre_norm=ops.Norm())[1]
     r, x = ops.residual_norm(h, pre_norm=ops.Norm(), out=(None, h))
     assert x is h and torch.equal(x, want) and torch.equal(r, was)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_operators_refuse_outputs_that_overlap(ops, dtype):
+    """Shifted, crossed, shared and differently laid out outputs; what lies between an input's rows, or is the input, is fine."""
+    freqs = ops.rotary_frequencies(64, device="cuda")[0]
+    packed = randn(31, 2, 9, 6, 64, dtype=dtype)
+    q, k, v = packed[:, :, :2], packed[:, :, 2:4], packed[:, :, 4:]
+    pos, lam = torch.arange(9, device="cuda"), torch.zeros(4, 32, device="cuda")
+    turn = lambda *out: ops.rotary(q, k, positions=pos, freqs=freqs, out=out)      # noqa: E731
+    h, y = (randn(s, 2, 8, 65, dtype=dtype) for s in (32, 33))
+    norm = lambda *out: ops.residual_norm(h[:, 1:, :64], y[:, 1:, :64], pre_norm=ops.Norm(), out=out)      # noqa: E731
+    before = packed.clone(), h.clone(), y.clone()
+    for call in [lambda: turn(k, q), lambda: turn(v, v), lambda: turn(q, packed[:, :, 1:3]), lambda: turn(packed[:, :, 1:3], None), lambda: turn(None, q),
+                 lambda: ops.diff_attention(q, k, v, lam, lambda_init=0.3, out=packed[:, :, 1:3]), lambda: ops.diff_attention(q, k, v, lam, lambda_init=0.3, out=v),
+                 lambda: norm(h[:, :7, :64], None), lambda: norm(h[:, 1:, 1:], None), lambda: norm(None, y[:, 1:, 1:]), lambda: norm(h[:, 1:, :64], h[:, 1:, :64]),
+                 lambda: norm(None, y[:, :7, :64])]:
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    assert torch.equal(packed, before[0]) and torch.equal(h, before[1]) and torch.equal(y, before[2])
+    want = ops.diff_attention(q, k, k, lam, lambda_init=0.3)
+    assert torch.equal(ops.diff_attention(q, k, k, lam, lambda_init=0.3, out=v), want)          # between the rows of q and k
+    want = turn(None, None)
+    got = turn(q, k)
+    assert got[0] is q and torch.equal(q, want[0]) and torch.equal(k, want[1])
+    want = norm(None, None)
+    r, x = norm(y[:, 1:, :64], h[:, 1:, :64])            # each over the other input
+    assert torch.equal(r, want[0]) and torch.equal(x, want[1])
