@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -123,6 +124,14 @@ def _call(name, argtypes, device, *args):
         _lib.check(rc, name)
 
 
+_NOT_PACKED = (struct.error, OverflowError)
+
+
+def _not_packed(args, e):
+    """What a struct does not take is a bad argument like any other."""
+    return ValueError(f"{args.__name__}: a size beyond 32 bits or an argument that is no number ({e})")
+
+
 _STREAM = (ctypes.c_void_p,)
 _WORKSPACE_STREAM = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p)
 
@@ -206,9 +215,13 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, positions: torc
     if hk:
         ks, kos, kp, kop = k.stride(), ko.stride(), k.data_ptr(), ko.data_ptr()
     qs, qos = q.stride(), qo.stride()
-    _call("rz_rotary", _STREAM, dev, _lib.RzRotaryArgs.pack(
-        _DTYPES[dt], _LAYOUT[layout], b, n, hq, hk, d, 2 * freqs.numel(), axes, amplitude, q.data_ptr(), qs[0], qs[1], qs[2], kp, ks[0], ks[1], ks[2],
-        qo.data_ptr(), qos[0], qos[1], qos[2], kop, kos[0], kos[1], kos[2], pos.data_ptr(), strides[0] if len(shape) == 2 else 0, strides[-1], freqs.data_ptr()))
+    try:
+        args = _lib.RzRotaryArgs.pack(
+            _DTYPES[dt], _LAYOUT[layout], b, n, hq, hk, d, 2 * freqs.numel(), axes, amplitude, q.data_ptr(), qs[0], qs[1], qs[2], kp, ks[0], ks[1], ks[2],
+            qo.data_ptr(), qos[0], qos[1], qos[2], kop, kos[0], kos[1], kos[2], pos.data_ptr(), strides[0] if len(shape) == 2 else 0, strides[-1], freqs.data_ptr())
+    except _NOT_PACKED as e:
+        raise _not_packed(_lib.RzRotaryArgs, e) from None
+    _call("rz_rotary", _STREAM, dev, args)
     if out is not None:
         _written(qo, ko)
     return qo if k is None else (qo, ko)
@@ -266,10 +279,14 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
         attention_mask, mask, mask_stride = x, x.data_ptr(), x.stride(0)
     given, out = out, _new(q) if out is None else _output(out, q.shape, dt, dev, "out")
     os = out.stride()
-    args = _lib.RzDiffAttentionArgs.pack(
-        _DTYPES[dt], b, h, hk, n_q, n_k, d, _CAUSAL[causal], d ** -0.5 if scale is None else scale, lambda_init, norm_eps, out_scale,
-        q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], out.data_ptr(), os[0], os[1], os[2],
-        lam, 4 * d if per_head else 0, _vector(norm_weight, "norm_weight", (w,), dev), lens, mask, mask_stride)
+    w_ptr = _vector(norm_weight, "norm_weight", (w,), dev)
+    try:
+        args = _lib.RzDiffAttentionArgs.pack(
+            _DTYPES[dt], b, h, hk, n_q, n_k, d, _CAUSAL[causal], d ** -0.5 if scale is None else scale, lambda_init, norm_eps, out_scale,
+            q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], out.data_ptr(), os[0], os[1], os[2],
+            lam, 4 * d if per_head else 0, w_ptr, lens, mask, mask_stride)
+    except _NOT_PACKED as e:
+        raise _not_packed(_lib.RzDiffAttentionArgs, e) from None
     need = _fn("rz_diff_attention_workspace")(args)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _call("rz_diff_attention", _WORKSPACE_STREAM, dev, args, ws.data_ptr() if need else 0, need)
@@ -341,9 +358,14 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
         batch, rows, hs, ys, rs, xs = 1, shape[0], (0, *hs), (0, *ys), (0, *rs), (0, *xs)
     else:
         batch, rows = shape[0], shape[1]
-    _call("rz_residual_norm", _STREAM, dev, _lib.RzResidualNormArgs.pack(
-        _DTYPES[t], _DTYPES[rt], batch, rows, dim, post_kind, pre_kind, alpha, post_eps, pre_eps, yp, ys[0], ys[1], residual.data_ptr(), hs[0], hs[1], rp, rs[0], rs[1],
-        xp, xs[0], xs[1], post_w, post_b, _vector(scale, "scale", (dim,), dev), gp, gb, gr, pre_w, pre_b))
+    scale_ptr = _vector(scale, "scale", (dim,), dev)
+    try:
+        args = _lib.RzResidualNormArgs.pack(
+            _DTYPES[t], _DTYPES[rt], batch, rows, dim, post_kind, pre_kind, alpha, post_eps, pre_eps, yp, ys[0], ys[1], residual.data_ptr(), hs[0], hs[1], rp, rs[0], rs[1],
+            xp, xs[0], xs[1], post_w, post_b, scale_ptr, gp, gb, gr, pre_w, pre_b)
+    except _NOT_PACKED as e:
+        raise _not_packed(_lib.RzResidualNormArgs, e) from None
+    _call("rz_residual_norm", _STREAM, dev, args)
     if out is not None:
         _written(*out)
     return ro, xo

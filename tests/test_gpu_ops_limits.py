@@ -221,3 +221,14 @@ def test_operators_refuse_outputs_that_overlap(ops, dtype):
     want = norm(None, None)
     r, x = norm(y[:, 1:, :64], h[:, 1:, :64])            # each over the other input
     assert torch.equal(r, want[0]) and torch.equal(x, want[1])
+
+
+def test_operators_refuse_arguments_beyond_their_fields(ops):
+    """Sizes of 2^31 (views without memory of their own) and what is no number are refused like any other bad argument.  (A factor beyond float32 is an infinity, as it is there.)"""
+    q, lam = torch.zeros(1, 1, 1, 64, device="cuda"), torch.zeros(4, 32, device="cuda")
+    pos, freqs = torch.zeros(1, dtype=torch.int64, device="cuda"), ops.rotary_frequencies(64, device="cuda")[0]
+    long, h = q.expand(1, 1 << 31, 1, 64), torch.zeros(2, 64, device="cuda")
+    for call in [lambda: ops.diff_attention(q, long, long, lam, lambda_init=0.3), lambda: ops.diff_attention(q, q, q, lam, lambda_init=0.3, out_scale=None),
+                 lambda: ops.rotary(q, positions=pos, freqs=freqs, amplitude="2"), lambda: ops.residual_norm(h, h, pre_norm=None, alpha=10 ** 400)]:
+        with pytest.raises(ValueError, match="Args"):
+            call()
