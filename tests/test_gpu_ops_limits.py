@@ -232,3 +232,26 @@ def test_operators_refuse_arguments_beyond_their_fields(ops):
                  lambda: ops.rotary(q, positions=pos, freqs=freqs, amplitude="2"), lambda: ops.residual_norm(h, h, pre_norm=None, alpha=10 ** 400)]:
         with pytest.raises(ValueError, match="Args"):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("axes", [1, 2])
+def test_rotary_at_the_farthest_positions(ops, dtype, layout, axes):
+    """One turn at positions from 2^24 to 2^31 of either sign, against cosines and sines of the angles in 64 bits.
+
+    The angle's product is the same in both.  The kernel then takes turns = angle / (2 pi), off by 2 roundings (the factor's and the product's) of at most 2^-53 of 2^31 / (2 pi)
+    turns: 2 2^-22 radian; the reference's cosine takes the angle as it is.  A fraction of a turn in fp32, its sine and cosine and three roundings: 5e-7."""
+    x = randn(41, 2, 300, 3, 64, dtype=dtype)
+    far = torch.randint(1 << 24, (1 << 31) - 1, (2, 300, axes), generator=torch.Generator(device="cuda").manual_seed(42), device="cuda")
+    far[0, :6, 0] = torch.tensor([(1 << 31) - 1, 1 << 30, (1 << 30) + 1, (1 << 24) + 1, 16777219, 2147483629], device="cuda")
+    far[1] *= -1
+    freqs, _ = ops.rotary_frequencies(64, axes=axes, device="cuda")
+    got = ops.rotary(x, positions=far if axes > 1 else far[..., 0], freqs=freqs, layout=layout).double()
+    angle = (far.double()[..., None] * freqs.view(axes, -1)).flatten(-2)[:, :, None]
+    pairs = (lambda t: (t[..., :32], t[..., 32:])) if layout == "half" else (lambda t: (t[..., 0::2], t[..., 1::2]))
+    u, w = pairs(x.double())
+    for y, ref in zip(pairs(got), (u * angle.cos() - w * angle.sin(), u * angle.sin() + w * angle.cos())):
+        tol = (5e-7 + 2 * 2.0 ** -22) * (u.abs() + w.abs())
+        tol = tol + U[dtype] * (ref.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0)
+        assert bool(((y - ref).abs() <= tol).all())
