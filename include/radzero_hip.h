@@ -265,7 +265,9 @@ int rz_rotary(const rz_rotary_args* args, void* stream);
  *   gets zeros.  What a hidden key holds, inf and NaN included, changes nothing.
  *   Statistics and sums are fp32; the 16-bit types round each weight exp(s - max) to the type for the product with v (f16, whose steps end: weights too
  *   small for it lose at most 2^-13 of a row's sum together, over up to 2^22 keys).  fp32 products may be taken from three bf16 parts
- *   of each operand (2^-22 |a||b| off); an infinity where a query sees it gives NaN.  out must not overlap the inputs.
+ *   of each operand (2^-22 |a||b| off, and 2^-126 of the other for values so small that a part of theirs ends there); an infinity where a query sees it
+ *   gives NaN.  A weight beside the first keys' may be up to 2^15 (f16: 2^16) before the sum is divided out: bf16 and fp32 values stay finite while
+ *   |v| * 2^15 * keys does.  out overlapping q, k or v is refused.
  *   workspace_dev: rz_diff_attention_workspace(args) bytes (0: may be NULL), 16-byte aligned, free for reuse when the call's kernels are done. */
 enum rz_causal { RZ_CAUSAL_NONE = 0, RZ_CAUSAL_START = 1, RZ_CAUSAL_END = 2 };
 typedef struct rz_diff_attention_args {

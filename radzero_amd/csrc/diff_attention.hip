@@ -699,9 +699,10 @@ template <typename T, int D> struct Out {
     }
 };
 
-// `l`: either map's sum of weights, 0 where the query sees no key.  Such a row is all zeros, and stays so where an eps of 0 would make its factor infinite.
-__device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, float sum_of_squares, float l) {
-    return !a.norm_weight_dev ? a.out_scale : l == 0.f ? 0.f : a.out_scale / sqrtf(sum_of_squares / (float)(2 * a.head_dim) + a.norm_eps);
+// `inverse`: 1 over the first map's sum of weights, 0 where the query sees no key.  Such a row is all zeros, and stays so where an eps of 0 would make its factor infinite.
+// (The sum itself in its place: 4 x 5330 tokens, bf16, 535 -> 542 us, other registers.)
+__device__ __forceinline__ float norm_factor(const rz_diff_attention_args& a, float sum_of_squares, float inverse) {
+    return !a.norm_weight_dev ? a.out_scale : inverse == 0.f ? 0.f : a.out_scale / sqrtf(sum_of_squares / (float)(2 * a.head_dim) + a.norm_eps);
 }
 
 template <typename T, int D, bool KEYS, typename F = Form<T, D, KEYS>>
@@ -1012,7 +1013,7 @@ __global__ __launch_bounds__(64 * F::W, F::kWaves) void diff_attention_kernel(co
         ss = 0.f;
         for (int w = 0; w < W; ++w) ss += stat[w * 32 + (lane & 31)];
     }
-    Out<T, D>::template store<OSTEP, OWN>(x, o[0], own0, at.b, i, head, live, norm_factor(a, ss, l[0]), h);
+    Out<T, D>::template store<OSTEP, OWN>(x, o[0], own0, at.b, i, head, live, norm_factor(a, ss, r[0]), h);
     return;                                                                // a whole unit is a workgroup's only piece
     }
 }
@@ -1028,7 +1029,7 @@ template <typename T, int D> __device__ __forceinline__ void finish_row(const Ar
         o[0][e] = o[0][e] * r0 - o[1][e] * r1;
         ss = fmaf(o[0][e], o[0][e], ss);
     }
-    const float f = norm_factor(a, wave_sum(ss), l0);
+    const float f = norm_factor(a, wave_sum(ss), r0);
     T* out = (T*)a.out_dev + b * a.out_batch_stride + i * a.out_token_stride + head * a.out_head_stride + lane * N;
 #pragma unroll
     for (int e = 0; e < N; ++e) out[e] = from_f32<T>(o[0][e] * f * (a.norm_weight_dev ? a.norm_weight_dev[lane * N + e] : 1.f));
@@ -1303,9 +1304,10 @@ int cu_count() {
     return n;
 }
 
-// Hardly any rows: no matrix unit.  us, with it / without, head dim 64: bf16, one row, 1 x 6 heads over 257 keys 12.8 / 10.4, 64 x 12 over 300 42 / 24; two rows 43 / 26, but
-// 8 x 4 over 300 12.8 / 15.7: only where every CU has a unit; four rows 43 / 56.  fp32, four rows, 8 x 4 over 8192 120 / 55;
-// eight (two blocks of four, each key read twice, by the same XCD), 64 x 12 over 300, head dims 32, 64, 128 60 / 68, 131 / 93, 215 / 197; twelve 60 / 104, 131 / 132, 216 / 240.
+// Hardly any rows: no matrix unit.  us, with it / without, three caches in turn, head dim 64: bf16, one row, 1 x 6 heads over 257 keys 11.9 / 10.4, 64 x 12 over 300 42 / 27; two
+// rows 42 / 30, but 8 x 4 over 300 11.9 / 15.5: only where every CU has a unit; four rows 43 / 60.  fp32, four rows, 8 x 4 over 8192 126 / 63; eight as two blocks of four, each
+// key read twice: 64 x 12 over 300, head dims 32, 64, 128 62 / 67, 133 / 93, 198 / 156, head dim 64 over long caches, 8 x 4 x 8192 126 / 82, 1 x 4 x 65536 132 / 96, 1 x 8 238 / 144
+// (the pieces of both blocks beside each other, on one XCD, change that by -3 .. +5 %); twelve, 64 x 12 over 300, 62 / 100, 133 / 142, 199 / 237.
 template <typename T, int D> bool few_form(const rz_diff_attention_args& a, int64_t rows) {
     return rows <= (sizeof(T) == 4 ? (D == 32 ? 4 : 8) : 1) || (rows == 2 && (int64_t)a.batch * a.kv_heads >= cu_count());
 }

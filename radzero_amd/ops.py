@@ -239,7 +239,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
     no key gets zeros; what hidden keys hold changes nothing.  norm_weight float32 (2 d): root-mean-square norm of every head's output.
     Sums and statistics are float32; the 16-bit types round each weight for the product with v (float16: weights too small for it lose at most 2^-13 of
     a row's sum together, over up to 2^22 keys); float32 products may be taken from three bf16 parts of each
-    operand (2^-22 of |a||b| off; an infinity that a query sees then gives NaN).
+    operand (2^-22 of |a||b| off, and 2^-126 of the other for values so small that a part of theirs ends there; an infinity that a query sees then gives NaN).
+    bfloat16 and float32 results are finite while |v| * 2^15 * keys is.
     16-byte alignment of q, k, v and out and of their strides is required.  Returns (batch, n_q, heads, 2 d), in `out` (no input's memory) if given."""
     if _differentiating():
         _no_tangents(q, k, v, lambda_qk, norm_weight)
