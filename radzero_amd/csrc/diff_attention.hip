@@ -14,10 +14,10 @@
 //   parts of every operand (rows), or 32x32x2, whose V^T fragments are plain reads of a row (keys).
 // Three ways to share the work:
 //   rows  4 waves x 32 rows on the same key tiles (16-bit: double-buffered in LDS, filled by LDS-DMA): many queries.  Bound by the matrix unit and the
-//         exponentials, whose times add on a SIMD: bf16, 4 x 5330 tokens, 6 heads of 64: 524 us, 1000 TFLOP/s executed (12 d per query and key)
+//         exponentials, whose times add on a SIMD: bf16, 4 x 5330 tokens, 6 heads of 64: 539 us, 970 TFLOP/s executed (12 d per query and key)
 //   keys  4 waves on the same 32 rows, every wave its own key tiles, joined in LDS: few queries over many keys.  Bound by HBM: 16 heads over 4 key heads, 8
 //         caches of 18432 .. 32768 tokens, bf16: 91 us, 4.6 TB/s
-//   few   a handful of rows without the matrix unit: fp32, 8 x 4 key heads x 8192 tokens: 52 us, 5.2 TB/s
+//   few   a handful of rows without the matrix unit: fp32, 8 x 4 key heads x 8192 tokens: 58 us, 4.6 TB/s
 // Each may also split the keys over workgroups; partial (O, m, l) then go through the workspace and a second kernel joins them.
 #include <atomic>
 #include <type_traits>
