@@ -1685,7 +1685,7 @@ struct Rows {
     }
 };
 
-// Whether two of them share an element.  A row of a begins D + (sum of e_i stride_i) bytes behind one of b, e_i over a range for every stride of either: the largest strides
+// Whether two of them share an element, or two rows of one do (given twice).  A row of a begins D + (sum of e_i stride_i) bytes behind one of b, e_i over a range for every stride of either: the largest strides
 // first, only those e_i from which the rest can still bring the two rows together (hardly ever more than two).  Given up, as apart, after 100000 steps.
 struct Meeting {
     __int128 stride[6], low[6], high[6], rest_low[7], rest_high[7], row_a, row_b;
@@ -1721,7 +1721,17 @@ static bool overlap(const Rows& a, const Rows& b) {
     }
     m.rest_low[m.terms] = m.rest_high[m.terms] = 0;
     for (int i = m.terms - 1; i >= 0; --i) m.rest_low[i] = m.rest_low[i + 1] + m.low[i] * m.stride[i], m.rest_high[i] = m.rest_high[i + 1] + m.high[i] * m.stride[i];
-    return m.from((__int128)(intptr_t)a.p - (__int128)(intptr_t)b.p, 0);
+    if (&a != &b) return m.from((__int128)(intptr_t)a.p - (__int128)(intptr_t)b.p, 0);
+    // a tensor and itself: two different rows, a step or more apart in the largest stride in which they differ
+    for (int i = 0; i < 3; ++i)
+        for (int j = 0; j <= i; ++j)
+            if (a.n[i] > 1 && a.n[j] > 1 && (a.stride[i] == 0 || (i != j && (a.stride[i] == a.stride[j] || a.stride[i] == -a.stride[j])))) return true;
+    for (int t = 0; t < m.terms; ++t) {
+        m.low[t] = 1, m.rest_low[t] = m.stride[t] + m.rest_low[t + 1];
+        if (m.from(0, t)) return true;
+        m.low[t] = -m.high[t];
+    }
+    return false;
 }
 
 int rz_rotary(const rz_rotary_args* a, void* stream) {
@@ -1743,6 +1753,7 @@ int rz_rotary(const rz_rotary_args* a, void* stream) {
     const Rows ko{a->k_out_dev, {a->batch, a->tokens, a->k_heads}, {a->k_out_batch_stride, a->k_out_token_stride, a->k_out_head_stride}, a->head_dim, size};
     if ((!qo.same(q) && overlap(qo, q)) || (!ko.same(k) && overlap(ko, k)) || overlap(qo, k) || overlap(ko, q) || overlap(qo, ko))
         return fail(RZ_ERR_INVALID, "rz_rotary: an output overlaps an input that it is not, or the other output");
+    if (overlap(qo, qo) || overlap(ko, ko)) return fail(RZ_ERR_INVALID, "rz_rotary: an output's rows overlap");
     if (!a->positions_dev || !a->freqs_dev) return fail(RZ_ERR_INVALID, "rz_rotary: null pointer");
     RZ_HIP(launch_rotary(*a, (hipStream_t)stream));
     return 0;
@@ -1784,6 +1795,7 @@ int rz_diff_attention(const rz_diff_attention_args* a, void* workspace, size_t w
         overlap(out, {a->k_dev, {a->batch, a->n_k, a->kv_heads}, {a->k_batch_stride, a->k_token_stride, a->k_head_stride}, cols, size}) ||
         overlap(out, {a->v_dev, {a->batch, a->n_k, a->kv_heads}, {a->v_batch_stride, a->v_token_stride, a->v_head_stride}, cols, size}))
         return fail(RZ_ERR_INVALID, "rz_diff_attention: out must not be q, k or v, or overlap them");
+    if (overlap(out, out)) return fail(RZ_ERR_INVALID, "rz_diff_attention: the rows of out overlap");
     RZ_HIP(launch_diff_attention(*a, workspace, (hipStream_t)stream));
     return 0;
 }
@@ -1808,6 +1820,7 @@ int rz_residual_norm(const rz_residual_norm_args* a, void* stream) {
         for (const Rows& o : {ro, xo})
             for (const Rows& i : {r, y})
                 if (!o.same(i) && overlap(o, i)) return fail(RZ_ERR_INVALID, "rz_residual_norm: an output overlaps an input that it is not");
+        if (overlap(ro, ro) || overlap(xo, xo)) return fail(RZ_ERR_INVALID, "rz_residual_norm: an output's rows overlap");
         if (overlap(ro, xo)) return fail(RZ_ERR_INVALID, "rz_residual_norm: the outputs overlap");
     }
     if (!a->y_dev && (a->post_kind || a->scale_dev || a->gate_dev)) return fail(RZ_ERR_INVALID, "rz_residual_norm: post norm, scale and gate need y");

@@ -235,7 +235,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lambda_qk:
     q (batch, n_q, heads, 2 d), k and v (batch, n_k, kv_heads, 2 d), d = 32, 64 or 128; a row of q and k is [first map | second map]; heads a multiple
     of kv_heads.  lambda_qk float32 (4, d) = lq1, lk1, lq2, lk2, or (heads, 4, d).  scale: 1 / sqrt(d) by default.
     causal: "start" = query i is token i and sees keys 0 .. i; "end" = the queries are the last n_q tokens of their sequence.
-    kv_lens integer (batch,): only the first kv_lens[b] keys count.  attention_mask (batch, n_k): 0 = hidden, as a tokenizer gives it.  A query that sees
+    kv_lens int32 or int64 (batch,): only the first kv_lens[b] keys count.  attention_mask integer or bool (batch, n_k): 0 = hidden, as a tokenizer gives it (int64 as it
+    is, other types through a copy).  A query that sees
     no key gets zeros; what hidden keys hold changes nothing.  norm_weight float32 (2 d): root-mean-square norm of every head's output.
     Sums and statistics are float32; the 16-bit types round each weight for the product with v (float16: weights too small for it lose at most 2^-13 of
     a row's sum together, over up to 2^22 keys); float32 products may be taken from three bf16 parts of each
@@ -337,7 +338,8 @@ def residual_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, p
         gb, gr = (0, 0) if gate.dim() == 1 else (st[0], st[1]) if gate.dim() == 3 else (st[0], 0) if nd == 3 else (0, st[0])
     ro, xo = (None, None) if out is None else out
     rp, rs, xp, xs = 0, (0, 0, 0), 0, (0, 0, 0)
-    if y is not None or alpha != 1.0 or ro is not None or pre_norm is None or (xo is not None and xo.data_ptr() == residual.data_ptr()):      # x over the residual: r is a copy
+    if y is not None or alpha != 1.0 or ro is not None or pre_norm is None or (isinstance(xo, torch.Tensor) and xo.data_ptr() == residual.data_ptr()):
+        # the last: x over the residual, r is a copy
         ro = _new(residual) if ro is None else _output(ro, shape, rt, dev, "out[0]")
         rp, rs = ro.data_ptr(), ro.stride()
     else:

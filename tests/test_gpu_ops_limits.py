@@ -255,3 +255,16 @@ def test_rotary_at_the_farthest_positions(ops, dtype, layout, axes):
         tol = (5e-7 + 2 * 2.0 ** -22) * (u.abs() + w.abs())
         tol = tol + U[dtype] * (ref.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0)
         assert bool(((y - ref).abs() <= tol).all())
+
+
+def test_operators_refuse_outputs_whose_rows_overlap(ops):
+    q, lam = randn(51, 2, 9, 2, 64), torch.zeros(4, 32, device="cuda")
+    pos, freqs = torch.arange(9, device="cuda"), ops.rotary_frequencies(64, device="cuda")[0]
+    windows = torch.zeros(10000, device="cuda").as_strided(q.shape, (1152, 64, 64, 1))
+    h = randn(52, 9, 64)
+    for call in [lambda: ops.rotary(q, positions=pos, freqs=freqs, out=windows), lambda: ops.diff_attention(q, q, q, lam, lambda_init=0.3, out=windows),
+                 lambda: ops.residual_norm(h, pre_norm=ops.Norm(), out=(None, torch.zeros(1000, device="cuda").as_strided((9, 64), (32, 1)))),
+                 lambda: ops.residual_norm(h, pre_norm=ops.Norm(), out=(None, "x"))]:
+        with pytest.raises(ValueError):
+            call()
+    assert bool((windows == 0).all())

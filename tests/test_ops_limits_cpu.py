@@ -78,6 +78,31 @@ def test_rotary_refuses_outputs_that_overlap(lib):
     assert min(found) > 500
 
 
+def test_rotary_refuses_outputs_whose_rows_overlap(lib):
+    """Random strides, equal ones among them, against a count of the bytes."""
+    r, found = random.Random(9), [0, 0]
+    for _ in range(4000):
+        n, cols, dtype = (r.randint(1, 4), r.randint(1, 4), r.randint(1, 3)), r.choice([2, 4, 8]), r.choice([0, 1])
+        s = [r.choice(STRIDES) for _ in n]
+        a = _lib.RzRotaryArgs(dtype=dtype, layout=0, batch=n[0], tokens=n[1], q_heads=n[2], k_heads=0, head_dim=cols, rotary_dim=2, n_axes=1, amplitude=1.0, q_dev=1 << 20, q_out_dev=4096,
+                              q_batch_stride=1024, q_token_stride=128, q_head_stride=16, q_out_batch_stride=s[0], q_out_token_stride=s[1], q_out_head_stride=s[2])
+        want = len(places(4096, n, s, cols, 4 >> dtype)) < n[0] * n[1] * n[2] * cols * (4 >> dtype)
+        assert lib.rz_rotary(ctypes.byref(a), None) == 10001
+        assert (b"rows overlap" in lib.rz_last_error()) == want, (n, cols, dtype, s)
+        found[want] += 1
+    assert min(found) > 500
+
+
+def test_other_outputs_whose_rows_overlap(lib):
+    a = _lib.RzDiffAttentionArgs(dtype=1, batch=1, heads=2, kv_heads=1, n_q=3, n_k=0, head_dim=32, scale=0.125, out_scale=1.0, q_dev=1 << 20, out_dev=4096, lambda_qk_dev=16,
+                                 out_batch_stride=0, out_token_stride=64, out_head_stride=128)
+    assert lib.rz_diff_attention(ctypes.byref(a), 16, 1 << 40, None) == 10001 and b"rows of out overlap" in lib.rz_last_error()
+    for name in ("resid_out", "out"):
+        a = _lib.RzResidualNormArgs(dtype=1, resid_dtype=0, batch=2, rows=3, dim=64, pre_kind=1, alpha=1.0, resid_dev=1 << 20, resid_batch_stride=192, resid_row_stride=64, scale_dev=16,
+                                    **{name + "_dev": 4096, name + "_batch_stride": 128, name + "_row_stride": 64})
+        assert lib.rz_residual_norm(ctypes.byref(a), None) == 10001 and b"rows overlap" in lib.rz_last_error()
+
+
 def test_residual_norm_refuses_outputs_that_overlap(lib):
     """The same for x beside a residual of another type (a scale without y ends the call where nothing overlaps)."""
     r, found = random.Random(8), [0, 0]
