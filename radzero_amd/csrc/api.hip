@@ -1685,8 +1685,9 @@ struct Rows {
     }
 };
 
-// Whether two of them share an element, or two rows of one do (given twice).  A row of a begins D + (sum of e_i stride_i) bytes behind one of b, e_i over a range for every stride of either: the largest strides
-// first, only those e_i from which the rest can still bring the two rows together (hardly ever more than two).  Given up, as apart, after 100000 steps.
+// Whether two of them share an element, or two rows of one do (given twice).  A row of a begins D + (sum of e_i stride_i) bytes behind one of b, e_i over a range for
+// every stride of either: the largest strides first, only those e_i from which the rest can still bring the two rows together (hardly ever more than two).  Given up,
+// as apart, after 100000 steps.
 struct Meeting {
     __int128 stride[6], low[6], high[6], rest_low[7], rest_high[7], row_a, row_b;
     int terms = 0, steps = 0;
